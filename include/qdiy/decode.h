@@ -146,6 +146,145 @@ int qd_lm_head_argmax(const uint16_t* x, const uint16_t* norm_w, float eps, cons
                       uint16_t* logits, int vocab, int hidden, void* workspace,
                       size_t workspace_bytes, int* token, hipStream_t stream);
 
+/* ---- Trees of drafted tokens ------------------------------------------------
+ *
+ * Speculative decoding over the KV cache; no counterpart in the reference,
+ * whose engine decodes one token per step.  A drafter proposes `nodes` tokens
+ * that form a tree: node 0 is the last emitted token (its K/V row is not in the
+ * cache yet), node t > 0 a drafted token that follows parents[t] < t.  One
+ * target step then checks all of them:
+ *
+ *   qd_tree_layout          (host, once per tree shape) masks and depths
+ *   per layer: projections of the nodes' rows (qd_gemm_nt), then
+ *     qd_tree_qkv_rope      bias, RoPE at prefix + depth, K/V rows of the nodes
+ *     qd_tree_attention     every node over the prefix and its ancestors
+ *   qd_tree_verify          which path stands, and the token after it
+ *   qd_tree_commit          that path's K/V rows into the caches of all layers
+ *
+ * The nodes' K/V rows lie apart from the cache, row t at base + t*tree_row_stride
+ * + head*tree_head_stride (elements), so a tree needs no cache rows of its own
+ * and the cache changes only when a path is committed.  The context's num_heads
+ * is the cache's head count; num_heads here is the number of query heads, a
+ * multiple of it: query head h reads cache head h / (num_heads / ctx heads).
+ * At most QD_TREE_MAX_NODES nodes.  Counts, depths and paths are device int32,
+ * so a step needs no host synchronisation before its next token is wanted.
+ * As for the other entry points, calls with distinct workspaces and outputs may
+ * run at the same time on several streams; a workspace belongs to one call
+ * at a time (two captured graphs that share one must not run together). */
+#define QD_TREE_MAX_NODES 1024
+
+/* Host only: masks and depths of a tree.  mask[t * ceil(nodes / 64) + w] bit b
+ * says whether node t sees node 64 w + b (itself and its ancestors); depth[0] is
+ * 0, depth[t] = depth[parents[t]] + 1.  parents[0] must be negative and
+ * 0 <= parents[t] < t otherwise (QD_EINVAL).  Either output may be NULL.  All
+ * three are host memory; copy the outputs to the device. */
+int qd_tree_layout(const int* parents, int nodes, uint64_t* mask, int* depth);
+
+/* QKV bias + rotate-half RoPE of a tree's nodes: for node t, with the
+ * arithmetic and the bits of qd_qkv_bias_rope_cache at position
+ * prefix + depth[t],
+ *   b = half(qkv[t] + bias)            (bias == NULL: b = qkv[t])
+ *   q_out[t] = rotated Q part, K row t of k_tree = rotated K part, V row t of
+ *   v_tree = V part of b.
+ * qkv rows are [num_heads + 2 * ctx heads][128] (Q, K, V), qkv_stride elements
+ * apart; q_out rows are [num_heads][128], q_stride apart.  qkv is not changed,
+ * unless q_out is qkv itself with the same stride (the Q part is then rotated in
+ * place).  depth is device memory, depth[t] >= 0; a node whose position lies
+ * outside [0, max_seqlen) gets NaN in all three rows, so that the mistake shows.
+ * All fp16 buffers 16-byte aligned, strides multiples of 8; depth 4-byte
+ * aligned; k_tree, v_tree and q_out must not overlap the inputs otherwise, nor
+ * q_out the node rows (QD_EINVAL). */
+int qd_tree_qkv_rope(qd_ctx* ctx, const uint16_t* qkv, long long qkv_stride, const uint16_t* bias,
+                     const int* depth, uint16_t* q_out, long long q_stride, uint16_t* k_tree,
+                     uint16_t* v_tree, long long tree_row_stride, long long tree_head_stride,
+                     int prefix, int nodes, int num_heads, int head_dim, hipStream_t stream);
+
+/* Attention of a tree's nodes, all heads:
+ *   out[t][h] = half( sum_j w_j V_j ),  w = softmax_j( q[t][h] . K_j / sqrt(128) )
+ * over the cache rows j < prefix and the node rows j whose bit is set in row t
+ * of mask (ceil(nodes / 64) words a row, device memory; any mask, not only
+ * qd_tree_layout's; bits past `nodes` are ignored).  A node that sees no row
+ * (prefix 0, no bit) gets zeros.  What K and V hold in rows that a node does not
+ * see, infinities and NaN too, does not reach its output.  fp32 accumulation on
+ * the matrix cores, softmax weights rounded to fp16 for the second product: not
+ * reproducible on the host, but the same bits from call to call.
+ * q and out rows are [num_heads][128], q_stride and out_stride elements apart.
+ * workspace: qd_tree_attention_workspace_bytes(ctx, nodes, num_heads) bytes of
+ * device memory, 16-byte aligned; its contents need not survive between calls.
+ * Requires 0 <= prefix <= max_seqlen; fp16 pointers 16-byte aligned, strides
+ * multiples of 8; mask 8-byte aligned; out and workspace overlap neither each
+ * other nor anything that is read (QD_EINVAL). */
+int qd_tree_attention(qd_ctx* ctx, const uint16_t* q, long long q_stride, const uint16_t* k_layer,
+                      const uint16_t* v_layer, const uint16_t* k_tree, const uint16_t* v_tree,
+                      long long tree_row_stride, long long tree_head_stride, const uint64_t* mask,
+                      uint16_t* out, long long out_stride, int prefix, int nodes, int num_heads,
+                      int head_dim, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* Workspace bytes of qd_tree_attention, at any prefix; 0 for arguments it
+ * refuses. */
+size_t qd_tree_attention_workspace_bytes(const qd_ctx* ctx, int nodes, int num_heads);
+
+/* Which drafted tokens stand.  target_logits row t (vocab halves, ldt elements
+ * apart) is the target's after node t, tokens[t] the node's token (tokens[0] is
+ * not read), parents as in qd_tree_layout.  From node 0 on, the current node's
+ * children are tested in index order; the first accepted one becomes the current
+ * node; when none is left one more token is taken and the walk ends:
+ *   temperature == 0 (greedy; the pointers u and draft_logits are not read):
+ *     child c stands if tokens[c] is the argmax of the current row; the last
+ *     token is the argmax.  Ties go to the lowest index, -0 equals +0, NaN
+ *     never wins (as qd_lm_head_argmax).
+ *   temperature > 0, draft_logits == NULL: with p = softmax(row / temperature),
+ *     child c stands if accept_u[c] * (sum of p) < p(tokens[c]); otherwise
+ *     p(tokens[c]) becomes 0.  (Drafts that are given tokens, e.g. the most
+ *     likely ones or copies from the prompt.)
+ *   temperature > 0 and draft_logits (row t: the drafter's logits after node t,
+ *     ldd apart; rows of nodes without children are not read), the children drawn
+ *     independently from q = softmax(draft row / temperature): child c stands if
+ *     accept_u[c] * q(tokens[c]) < p(tokens[c]); otherwise p becomes
+ *     max(p - q, 0), normalised.  Only the first max_children children of a
+ *     node are tested (1 <= max_children <= 64; not read in the other modes).
+ *   The last token of the two sampled modes is the first index whose cumulative
+ *   p exceeds sample_u[0] times its total.
+ * In both sampled modes the emitted tokens are distributed as the target's when
+ * accept_u and sample_u are independent uniforms of [0, 1).  Weights are held
+ * and summed in 64 bits.  A NaN logit counts as -inf; +inf logits share the
+ * whole probability; a row of -inf alone is uniform.  A token outside
+ * [0, vocab) is never accepted, a node whose parent is not in [0, t) never
+ * reached.  If max(p - q, 0) is zero everywhere, p is kept as it was.
+ *   path[nodes]:    the accepted nodes from node 0 on, then -1
+ *   emitted[nodes]: the tokens of path[1..], then the last token, then -1
+ *   count[0]:       the number of entries of both (1 + accepted drafts)
+ * tokens, parents, u and the outputs are device memory, 4-byte aligned; logits
+ * 2-byte aligned, ldt and ldd >= vocab.  workspace: device memory, 16-byte
+ * aligned, of qd_tree_verify_workspace_bytes(nodes, vocab, max_children) bytes.
+ * Outputs and workspace overlap neither each other nor anything that is read
+ * (QD_EINVAL). */
+int qd_tree_verify(const uint16_t* target_logits, long long ldt, const uint16_t* draft_logits,
+                   long long ldd, const int* tokens, const int* parents, const float* accept_u,
+                   const float* sample_u, float temperature, int nodes, int vocab,
+                   int max_children, void* workspace, size_t workspace_bytes, int* path,
+                   int* emitted, int* count, hipStream_t stream);
+
+/* Workspace bytes of qd_tree_verify in any mode; 0 for arguments it refuses. */
+size_t qd_tree_verify_workspace_bytes(int nodes, int vocab, int max_children);
+
+/* Copies the K/V rows of an accepted path into the caches of all layers: for
+ * every layer l and i < count[0], cache row prefix + i = node row path[i].
+ * Layer l of the node rows starts at k_tree + l*tree_layer_stride, of the caches
+ * at k_cache + l*cache_layer_stride (elements; v alike).  path and count are
+ * device memory (qd_tree_verify's); entries outside [0, nodes), rows at or past
+ * max_seqlen and entries from `nodes` on are skipped; other rows are left as they
+ * were.  The node rows may be the cache's own rows from prefix on, in every layer
+ * (k_tree == k_cache + prefix*kv_row_stride, v alike, all strides the caches'),
+ * with path ascending: the path's rows are then moved up in place.  Otherwise
+ * they must not overlap the caches (QD_EINVAL).  fp16 pointers 16-byte aligned,
+ * strides multiples of 8. */
+int qd_tree_commit(qd_ctx* ctx, const uint16_t* k_tree, const uint16_t* v_tree,
+                   long long tree_layer_stride, long long tree_row_stride,
+                   long long tree_head_stride, uint16_t* k_cache, uint16_t* v_cache,
+                   long long cache_layer_stride, const int* path, const int* count, int prefix,
+                   int nodes, int layers, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

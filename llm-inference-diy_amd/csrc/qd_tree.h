@@ -1,0 +1,82 @@
+// Launch parameters of the drafted-token tree kernels (qd_tree_attention.hip,
+// qd_tree_rows.hip, qd_tree_verify.hip), between them and the C ABI (qd_tree.cpp).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+namespace qd {
+
+// Rows of a tree's nodes, and of the cache they follow.  Strides in halves.
+struct TreeRopeParams {
+  const uint16_t* qkv;      // [nodes][(heads + 2 kv_heads) * 128]
+  const uint16_t* bias;     // [(heads + 2 kv_heads) * 128] or null
+  const int* depth;
+  uint16_t* q_out;
+  uint16_t* k_tree;
+  uint16_t* v_tree;
+  const float2* rope_cs;    // [max_seqlen][64] (cos, sin)
+  long long qkv_stride, q_stride, row_stride, head_stride;
+  int prefix, nodes, heads, kv_heads, max_seqlen;
+};
+hipError_t launch_tree_rope(const TreeRopeParams& p, hipStream_t stream);
+
+struct TreeCommitParams {
+  const uint16_t* src[2];   // node rows of K and of V
+  uint16_t* dst[2];         // the caches
+  long long src_layer, src_row, src_head;
+  long long dst_layer, dst_row, dst_head;
+  const int* path;
+  const int* count;
+  int prefix, nodes, layers, kv_heads, max_seqlen;
+  int in_place;             // the node rows are the cache's own from prefix on
+};
+hipError_t launch_tree_commit(const TreeCommitParams& p, hipStream_t stream);
+
+struct TreeAttnParams {
+  const uint16_t* q;        // [nodes][heads][128]
+  const uint16_t* k;        // cache rows [0, prefix)
+  const uint16_t* v;
+  const uint16_t* kt;       // node rows
+  const uint16_t* vt;
+  const uint64_t* mask;     // [nodes][ceil(nodes / 64)]
+  uint16_t* out;
+  long long q_stride, out_stride;
+  long long row_stride, head_stride;      // cache
+  long long trow_stride, thead_stride;    // node rows
+  int prefix, nodes, heads, kv_heads;
+  float scale_log2;         // log2(e) / sqrt(128)
+};
+hipError_t launch_tree_attention(const TreeAttnParams& p, hipStream_t stream);
+
+// Logits of a row per workgroup of the verification's passes over them.
+constexpr int kVerifyChunk = 8192;
+inline int verify_chunks(int vocab) { return (vocab + kVerifyChunk - 1) / kVerifyChunk; }
+
+struct TreeVerifyParams {
+  const uint16_t* target;   // [nodes][vocab]
+  const uint16_t* draft;    // the drafter's, or null
+  const int* tokens;
+  const int* parents;
+  const float* accept_u;
+  const float* sample_u;
+  int* path;
+  int* emitted;
+  int* count;
+  // Workspace: per side (target, draft), node and chunk the largest logit and
+  // the chunk's sum of weights relative to it (greedy: the argmax and its
+  // logit); then per round, node and chunk the sums of max(p - A q, 0).
+  double* sums;             // [2][nodes][chunks]
+  double* rounds;           // [max_children][nodes][chunks]
+  float* maxes;             // [2][nodes][chunks]
+  int* args;                // [nodes][chunks]
+  long long ldt, ldd;
+  double scale_log2;        // log2(e) / temperature
+  int nodes, vocab, chunks, max_children;
+  int greedy;
+};
+hipError_t launch_tree_verify(const TreeVerifyParams& p, hipStream_t stream);
+
+}  // namespace qd

@@ -38,6 +38,8 @@ EXPORTS = (
     # qdiy/decode.h
     "qd_proj_residual", "qd_ffn_up_swiglu", "qd_lm_head_workspace_bytes", "qd_lm_head_argmax",
     "qd_gemm_nt", "qd_gemm_swiglu", "qd_prefill_attention",
+    "qd_tree_layout", "qd_tree_qkv_rope", "qd_tree_attention", "qd_tree_attention_workspace_bytes",
+    "qd_tree_verify", "qd_tree_verify_workspace_bytes", "qd_tree_commit",
     # qdiy/engine.h
     "qd_model_image_bytes", "qd_model_fill_random", "qd_model_write_random", "qd_engine_create",
     "qd_engine_create_from_image", "qd_engine_destroy", "qd_engine_config", "qd_engine_reset",
@@ -138,6 +140,17 @@ def load() -> ctypes.CDLL:
     L.qd_lm_head_workspace_bytes.argtypes = [i]
     L.qd_lm_head_workspace_bytes.restype = ctypes.c_size_t
     L.qd_lm_head_argmax.argtypes = [vp, vp, ctypes.c_float, vp, vp, i, i, vp, ctypes.c_size_t, vp, vp]
+    f = ctypes.c_float
+    L.qd_tree_layout.argtypes = [ip, i, ctypes.POINTER(ctypes.c_uint64), ip]
+    L.qd_tree_qkv_rope.argtypes = [vp, vp, ll, vp, vp, vp, ll, vp, vp, ll, ll, i, i, i, i, vp]
+    L.qd_tree_attention.argtypes = [vp, vp, ll, vp, vp, vp, vp, ll, ll, vp, vp, ll, i, i, i, i, vp,
+                                    ctypes.c_size_t, vp]
+    L.qd_tree_attention_workspace_bytes.argtypes = [vp, i, i]
+    L.qd_tree_attention_workspace_bytes.restype = ctypes.c_size_t
+    L.qd_tree_verify.argtypes = [vp, ll, vp, ll, vp, vp, vp, vp, f, i, i, i, vp, ctypes.c_size_t, vp, vp, vp, vp]
+    L.qd_tree_verify_workspace_bytes.argtypes = [i, i, i]
+    L.qd_tree_verify_workspace_bytes.restype = ctypes.c_size_t
+    L.qd_tree_commit.argtypes = [vp, vp, vp, ll, ll, ll, vp, vp, ll, vp, vp, i, i, i, vp]
     L.qd_model_image_bytes.argtypes = [ctypes.POINTER(ModelCfg)]
     L.qd_model_image_bytes.restype = ll
     L.qd_model_fill_random.argtypes = [vp, ll, ctypes.POINTER(ModelCfg), ctypes.c_uint64,
@@ -197,6 +210,31 @@ def _ptr(t: torch.Tensor, name: str, contiguous: bool = True) -> int:
     if not t.is_cuda:
         raise ValueError(f"{name} must be a GPU tensor")
     raise ValueError(f"{name} must be contiguous")
+
+
+def _typed_ptr(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int) -> int:
+    """The address of a contiguous GPU tensor of `dtype` with at least `numel` elements."""
+    if not isinstance(t, _Tensor) or t.dtype is not dtype:
+        raise TypeError(f"{name} must be a {dtype} torch.Tensor")
+    if not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous GPU tensor")
+    if t.numel() < numel:
+        raise ValueError(f"{name} holds {t.numel()} elements, needs {numel}")
+    return t.data_ptr()
+
+
+def _workspace(t: torch.Tensor) -> tuple:
+    if not isinstance(t, _Tensor) or not t.is_cuda or not t.is_contiguous():
+        raise TypeError("workspace must be a contiguous GPU tensor")
+    return t.data_ptr(), t.numel() * t.element_size()
+
+
+def _on_one_device(*tensors) -> None:
+    """Kernels run on the current device: tensors of another one are refused."""
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"a tensor is on device {t.get_device()}, the current device is {dev}")
 
 
 class Context:
@@ -417,6 +455,103 @@ class Context:
                                              _ptr(v_layer, "v_layer", False), pos, max_seqlen, H,
                                              HEAD_DIM, _stream(stream)))
 
+    # -- trees of drafted tokens -------------------------------------------------
+    def _check_rows(self, t: torch.Tensor, name: str, rows: int, row: int, head: int, base: int = 0) -> None:
+        last = base + (rows - 1) * row + (self.num_heads - 1) * head + HEAD_DIM
+        if rows >= 1 and t.numel() < last:
+            raise ValueError(f"{name} holds {t.numel()} elements; {rows} rows need {last}")
+
+    def tree_qkv_rope(self, qkv: torch.Tensor, bias, depth: torch.Tensor, q_out: torch.Tensor,
+                      k_tree: torch.Tensor, v_tree: torch.Tensor, prefix: int, nodes: int,
+                      num_heads: int | None = None, qkv_stride: int | None = None,
+                      q_stride: int | None = None, tree_row_stride: int | None = None,
+                      tree_head_stride: int = HEAD_DIM, stream=None) -> None:
+        """qd_tree_qkv_rope: bias and RoPE of a drafted tree's nodes at prefix + depth; the
+        rotated Q rows into q_out, the nodes' K/V rows into k_tree and v_tree."""
+        H, KH = self.num_heads if num_heads is None else num_heads, self.num_heads
+        row = (H + 2 * KH) * HEAD_DIM
+        qkv_stride = row if qkv_stride is None else qkv_stride
+        q_stride = H * HEAD_DIM if q_stride is None else q_stride
+        tree_row_stride = KH * HEAD_DIM if tree_row_stride is None else tree_row_stride
+        if qkv.numel() < (nodes - 1) * qkv_stride + row or q_out.numel() < (nodes - 1) * q_stride + H * HEAD_DIM:
+            raise ValueError("qkv or q_out too small for nodes, num_heads and the strides")
+        if bias is not None and bias.numel() < row:
+            raise ValueError(f"bias needs {row} elements")
+        self._check_rows(k_tree, "k_tree", nodes, tree_row_stride, tree_head_stride)
+        self._check_rows(v_tree, "v_tree", nodes, tree_row_stride, tree_head_stride)
+        _on_one_device(qkv, bias, depth, q_out, k_tree, v_tree)
+        _check(load().qd_tree_qkv_rope(self._h, _ptr(qkv, "qkv"), qkv_stride,
+                                       None if bias is None else _ptr(bias, "bias"),
+                                       _typed_ptr(depth, "depth", torch.int32, nodes), _ptr(q_out, "q_out"),
+                                       q_stride, _ptr(k_tree, "k_tree"), _ptr(v_tree, "v_tree"),
+                                       tree_row_stride, tree_head_stride, prefix, nodes, H, HEAD_DIM,
+                                       _stream(stream)))
+
+    def tree_attention_workspace_bytes(self, nodes: int, num_heads: int | None = None) -> int:
+        """qd_tree_attention_workspace_bytes: enough at any prefix."""
+        n = load().qd_tree_attention_workspace_bytes(self._h, nodes, self.num_heads if num_heads is None else num_heads)
+        if n == 0:
+            _check(QD_EINVAL)
+        return n
+
+    def tree_attention(self, q: torch.Tensor, k_layer: torch.Tensor, v_layer: torch.Tensor,
+                       k_tree: torch.Tensor, v_tree: torch.Tensor, mask: torch.Tensor, out: torch.Tensor,
+                       prefix: int, nodes: int, workspace: torch.Tensor, num_heads: int | None = None,
+                       q_stride: int | None = None, out_stride: int | None = None,
+                       tree_row_stride: int | None = None, tree_head_stride: int = HEAD_DIM,
+                       stream=None) -> torch.Tensor:
+        """qd_tree_attention: node t of a drafted tree attends over the cache rows [0, prefix)
+        and the node rows whose bit is set in row t of mask (int64 words)."""
+        H, KH = self.num_heads if num_heads is None else num_heads, self.num_heads
+        row = H * HEAD_DIM
+        q_stride = row if q_stride is None else q_stride
+        out_stride = row if out_stride is None else out_stride
+        tree_row_stride = KH * HEAD_DIM if tree_row_stride is None else tree_row_stride
+        if q.numel() < (nodes - 1) * q_stride + row or out.numel() < (nodes - 1) * out_stride + row:
+            raise ValueError("q and out need (nodes-1)*stride + num_heads*128 elements")
+        if 0 <= prefix <= self.max_seqlen:
+            self._check_rows(k_layer, "k_layer", prefix, self.kv_row_stride, self.kv_head_stride)
+            self._check_rows(v_layer, "v_layer", prefix, self.kv_row_stride, self.kv_head_stride)
+        self._check_rows(k_tree, "k_tree", nodes, tree_row_stride, tree_head_stride)
+        self._check_rows(v_tree, "v_tree", nodes, tree_row_stride, tree_head_stride)
+        _on_one_device(q, k_layer, v_layer, k_tree, v_tree, mask, out, workspace)
+        ws, ws_bytes = _workspace(workspace)
+        _check(load().qd_tree_attention(self._h, _ptr(q, "q"), q_stride, _ptr(k_layer, "k_layer"),
+                                        _ptr(v_layer, "v_layer"), _ptr(k_tree, "k_tree"), _ptr(v_tree, "v_tree"),
+                                        tree_row_stride, tree_head_stride,
+                                        _typed_ptr(mask, "mask", torch.int64, nodes * ((nodes + 63) // 64)),
+                                        _ptr(out, "out"), out_stride, prefix, nodes, H, HEAD_DIM, ws, ws_bytes,
+                                        _stream(stream)))
+        return out
+
+    def tree_commit(self, k_tree: torch.Tensor, v_tree: torch.Tensor, k_cache: torch.Tensor,
+                    v_cache: torch.Tensor, path: torch.Tensor, count: torch.Tensor, prefix: int, nodes: int,
+                    layers: int = 1, tree_layer_stride: int | None = None, tree_row_stride: int | None = None,
+                    tree_head_stride: int = HEAD_DIM, cache_layer_stride: int | None = None,
+                    stream=None) -> None:
+        """qd_tree_commit: the path's node rows into cache rows prefix, prefix + 1, ... of all
+        layers.  Layers are numel // layers elements apart by default."""
+        if layers < 1:
+            raise ValueError("layers must be >= 1")
+        tree_row_stride = self.num_heads * HEAD_DIM if tree_row_stride is None else tree_row_stride
+        tl = k_tree.numel() // layers if tree_layer_stride is None else tree_layer_stride
+        cl = k_cache.numel() // layers if cache_layer_stride is None else cache_layer_stride
+        if tree_layer_stride is None and v_tree.numel() != k_tree.numel():
+            raise ValueError("k_tree and v_tree differ in size: give tree_layer_stride")
+        if cache_layer_stride is None and v_cache.numel() != k_cache.numel():
+            raise ValueError("k_cache and v_cache differ in size: give cache_layer_stride")
+        for t, name in ((k_tree, "k_tree"), (v_tree, "v_tree")):
+            self._check_rows(t, name, nodes, tree_row_stride, tree_head_stride, (layers - 1) * tl)
+        for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+            self._check_rows(t, name, min(self.max_seqlen, max(0, prefix) + nodes), self.kv_row_stride,
+                             self.kv_head_stride, (layers - 1) * cl)
+        _on_one_device(k_tree, v_tree, k_cache, v_cache, path, count)
+        _check(load().qd_tree_commit(self._h, _ptr(k_tree, "k_tree", False), _ptr(v_tree, "v_tree", False), tl,
+                                     tree_row_stride, tree_head_stride, _ptr(k_cache, "k_cache"),
+                                     _ptr(v_cache, "v_cache"), cl, _typed_ptr(path, "path", torch.int32, nodes),
+                                     _typed_ptr(count, "count", torch.int32, 1), prefix, nodes, layers,
+                                     _stream(stream)))
+
 
 def xcd_placement(count: int = 256) -> list:
     """qd_xcd_placement: the XCD each workgroup of one count-workgroup launch ran on."""
@@ -517,6 +652,52 @@ def lm_head_argmax(x: torch.Tensor, norm_w: torch.Tensor, w: torch.Tensor, logit
     _check(load().qd_lm_head_argmax(_ptr(x, "x"), _ptr(norm_w, "norm_w"), eps, _ptr(w, "w"),
                                     _ptr(logits, "logits"), vocab, hidden,
                                     workspace.data_ptr(), ws, token.data_ptr(), _stream(stream)))
+
+
+def tree_layout(parents) -> tuple:
+    """qd_tree_layout: (mask int64 [nodes][ceil(nodes / 64)], depth int32 [nodes]) of a drafted
+    tree as CPU tensors; parents[0] is negative, parents[t] < t."""
+    n = len(parents)
+    par = (ctypes.c_int * max(1, n))(*parents)
+    mask = torch.empty((n, (n + 63) // 64), dtype=torch.int64)
+    depth = torch.empty(n, dtype=torch.int32)
+    _check(load().qd_tree_layout(par, n, ctypes.cast(mask.data_ptr(), ctypes.POINTER(ctypes.c_uint64)),
+                                 ctypes.cast(depth.data_ptr(), ctypes.POINTER(ctypes.c_int))))
+    return mask, depth
+
+
+def tree_verify_workspace_bytes(nodes: int, vocab: int, max_children: int = 0) -> int:
+    """qd_tree_verify_workspace_bytes: enough in any mode."""
+    n = load().qd_tree_verify_workspace_bytes(nodes, vocab, max_children)
+    if n == 0:
+        raise ValueError(f"nodes {nodes}, vocab {vocab} or max_children {max_children} out of range")
+    return n
+
+
+def tree_verify(target_logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, nodes: int,
+                vocab: int, workspace: torch.Tensor, path: torch.Tensor, emitted: torch.Tensor,
+                count: torch.Tensor, temperature: float = 0.0, accept_u: torch.Tensor | None = None,
+                sample_u: torch.Tensor | None = None, draft_logits: torch.Tensor | None = None,
+                max_children: int = 0, ldt: int | None = None, ldd: int | None = None, stream=None) -> None:
+    """qd_tree_verify: which path of a drafted tree stands against the target's logits, and the
+    token after it; greedy at temperature 0, else from the given uniforms accept_u and sample_u."""
+    ldt = vocab if ldt is None else ldt
+    ldd = vocab if ldd is None else ldd
+    if target_logits.numel() < (nodes - 1) * ldt + vocab:
+        raise ValueError("target_logits too small for nodes, vocab and ldt")
+    if draft_logits is not None and draft_logits.numel() < (nodes - 1) * ldd + vocab:
+        raise ValueError("draft_logits too small for nodes, vocab and ldd")
+    _on_one_device(target_logits, draft_logits, tokens, parents, accept_u, sample_u, workspace, path, emitted, count)
+    ws, ws_bytes = _workspace(workspace)
+    i32, f32 = torch.int32, torch.float32
+    _check(load().qd_tree_verify(
+        _ptr(target_logits, "target_logits"), ldt,
+        None if draft_logits is None else _ptr(draft_logits, "draft_logits"), ldd,
+        _typed_ptr(tokens, "tokens", i32, nodes), _typed_ptr(parents, "parents", i32, nodes),
+        None if accept_u is None else _typed_ptr(accept_u, "accept_u", f32, nodes),
+        None if sample_u is None else _typed_ptr(sample_u, "sample_u", f32, 1), temperature, nodes, vocab,
+        max_children, ws, ws_bytes, _typed_ptr(path, "path", i32, nodes),
+        _typed_ptr(emitted, "emitted", i32, nodes), _typed_ptr(count, "count", i32, 1), _stream(stream)))
 
 
 # ---------------------------------------------------------------- engine.h
