@@ -48,8 +48,33 @@ struct TreeAttnParams {
   long long trow_stride, thead_stride;    // node rows
   int prefix, nodes, heads, kv_heads;
   float scale_log2;         // log2(e) / sqrt(128)
+  int splits;               // workgroups per block of query rows (TreeAttnPlan)
+  float* part_o;            // [kv_heads][nodes * group][splits][128], when splits > 1
+  float2* part_ml;          // [kv_heads][nodes * group][splits] (log2 reference, denominator)
 };
-hipError_t launch_tree_attention(const TreeAttnParams& p, hipStream_t stream);
+
+// Launch plan: blocks of 16 * q_tiles query rows per cache head (a cache head's query rows
+// are its nodes x heads that share it), `splits` workgroups of `waves` waves for each.
+struct TreeAttnPlan {
+  int q_tiles, waves, blocks, splits;
+};
+constexpr int kTreeWaves1 = 8, kTreeWaves2 = 8, kTreeWaves4 = 4;
+
+// max_splits: what the workspace is sized for, at any prefix.
+inline TreeAttnPlan tree_attn_plan(int nodes, int heads, int kv_heads, int prefix, int num_cus, int* max_splits) {
+  TreeAttnPlan plan;
+  const int rows = nodes * (heads / kv_heads);
+  plan.q_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  plan.waves = plan.q_tiles == 1 ? kTreeWaves1 : plan.q_tiles == 2 ? kTreeWaves2 : kTreeWaves4;
+  plan.blocks = (rows + 16 * plan.q_tiles - 1) / (16 * plan.q_tiles);
+  const int most = num_cus / (plan.blocks * kv_heads);
+  *max_splits = most < 1 ? 1 : most;
+  const int tiles = (prefix + 31) / 32 + (nodes + 31) / 32;
+  const int by_tiles = (tiles + plan.waves - 1) / plan.waves;
+  plan.splits = *max_splits < by_tiles ? *max_splits : by_tiles;
+  return plan;
+}
+hipError_t launch_tree_attention(const TreeAttnParams& p, const TreeAttnPlan& plan, hipStream_t stream);
 
 // Logits of a row per workgroup of the verification's passes over them.
 constexpr int kVerifyChunk = 8192;

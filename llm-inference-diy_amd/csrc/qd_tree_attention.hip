@@ -1,4 +1,30 @@
-// Attention of a tree of drafted tokens over a KV cache (gfx950).
+// Attention of a tree of drafted tokens over a KV cache, on the matrix cores (gfx950
+// v_mfma_f32_16x16x32_f16).
+//
+// The query rows of one cache head -- `nodes` times the query heads that share it -- are
+// handled together, so every K/V row is read once for up to 64 of them; with few rows a step
+// is bound by the cache's bytes.  The keys form tiles of 32 rows: those of the cache, then the
+// node rows, which alone are masked.  A workgroup takes one block of 16 kQ query rows of one
+// cache head and every splits-th group of kW tiles, a tile per wave; its waves keep a softmax
+// state each over all of the block's rows and are folded through LDS at the end.  Several
+// splits leave fp32 partials in the workspace, which a second launch folds.
+//
+// Nothing goes through LDS on the way to the products:
+//   S^T = K Q^T     (M = 16 keys, two tiles; N = 16 queries; K = 128 dims in four steps)
+//   O^T += V^T P^T  (M = 16 dims, eight tiles; N = 16 queries; K = 32 keys)
+// Operand lanes (c = l % 16, g = l / 16): A[c][8 g + e], B[8 g + e][c]; accumulator
+// D[4 g + r][c].  K rows feed A as loaded, 16 bytes a lane.  S^T leaves lane (g, c) the
+// scores of keys 16 a + 4 g + r of query c, which become P^T's B operand in place: its slot
+// 8 g + 4 a + r stands for key 16 a + 4 g + r.  V^T's A operand then needs, per dim, those
+// eight keys: a lane loads dims 8 c .. 8 c + 7 of its group's eight V rows (an instruction
+// reads four whole rows) and transposes the 8 x 8 halves with 32 byte permutations; the dims
+// tile e takes dim 8 c + e of every lane, so lane (g, c) ends with dims 32 g .. 32 g + 31 of
+// query c, and stores rows of its own.
+//
+// Weights are rounded to fp16 for the second product, and the denominator sums the rounded
+// weights on the matrix core (an all-ones A operand), so an output is a weighted mean of V
+// rows.  A query's reference maximum moves only when a score passes it by more than 2^kLazy:
+// weights stay below 2^kLazy, and the accumulators are scaled in few tiles.
 #include "qd_device.h"
 #include "qd_internal.h"
 #include "qd_tree.h"
@@ -6,55 +32,339 @@
 namespace qd {
 namespace {
 
-// One workgroup per (node, head); its four waves take rows in turn.  Lane l
-// holds dims 2 l and 2 l + 1.
-__global__ __launch_bounds__(256) void tree_attention_kernel(TreeAttnParams p) {
-  __shared__ float so[4][128], sm[4], sl[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int h = blockIdx.x % p.heads, t = blockIdx.x / p.heads;
-  const int kh = h / (p.heads / p.kv_heads);
+constexpr int kKeys = 32;
+constexpr float kLazy = 8.0f;            // log2 of the largest softmax weight before a rescale
+constexpr int kFoldRow = 132;            // floats of a query's O row in LDS: 128, and 4 to spread the banks
+__device__ constexpr float kNone = -__builtin_inff();
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+// Eight keys x eight dims of V as loaded, row 4 a + i of the group: va[e] slot 4 a + i is its
+// dim e.
+__device__ __forceinline__ f16x8 v_column(const u32x4 (&v)[8], int e) {
+  u32x4 r;
+  const unsigned sel = e & 1 ? 0x07060302u : 0x05040100u;   // high or low halves of (second, first)
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r[j] = __builtin_amdgcn_perm(v[2 * j + 1][e >> 1], v[2 * j][e >> 1], sel);
+  return __builtin_bit_cast(f16x8, r);
+}
+
+__device__ __forceinline__ bool any_nonfinite(const u32x4 (&v)[8]) {
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[i][j] & 0x7fff7fffu));
+  return m[0] >= 0x7c00 || m[1] >= 0x7c00;
+}
+
+template <int kQ, int kW>
+__global__ __launch_bounds__(kW * 64) void tree_attention_kernel(TreeAttnParams p) {
+  __shared__ __align__(16) float fold_o[kW][16 * kQ][kFoldRow];
+  __shared__ float fold_m[kW][16 * kQ], fold_l[kW][16 * kQ];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int split = blockIdx.x % p.splits;
+  const int kh = (blockIdx.x / p.splits) % p.kv_heads;
+  const int r0 = (blockIdx.x / p.splits / p.kv_heads) * 16 * kQ;   // the block's first query row
+  const int group = p.heads / p.kv_heads;
+  const int rows = p.nodes * group;
+  const int cache_tiles = (p.prefix + kKeys - 1) / kKeys;
+  const int tiles = cache_tiles + (p.nodes + kKeys - 1) / kKeys;
   const int words = (p.nodes + 63) / 64;
-  const f16x2 qv = *reinterpret_cast<const f16x2*>(p.q + t * p.q_stride + h * 128 + 2 * lane);
-  float m = -__builtin_inff(), l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-  for (int j = wave; j < p.prefix + p.nodes; j += 4) {
-    const int n = j - p.prefix;
-    if (n >= 0 && !((p.mask[(long long)t * words + n / 64] >> (n % 64)) & 1)) continue;
-    const uint16_t* k = n < 0 ? p.k + j * p.row_stride + kh * p.head_stride : p.kt + n * p.trow_stride + kh * p.thead_stride;
-    const uint16_t* v = n < 0 ? p.v + j * p.row_stride + kh * p.head_stride : p.vt + n * p.trow_stride + kh * p.thead_stride;
-    const f16x2 kv = *reinterpret_cast<const f16x2*>(k + 2 * lane);
-    const f16x2 vv = *reinterpret_cast<const f16x2*>(v + 2 * lane);
-    const float s = wave64_sum((float)qv[0] * (float)kv[0] + (float)qv[1] * (float)kv[1]) * p.scale_log2;
-    const float mn = fmaxf(m, s);
-    const float a = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-    const float w = mn == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(s - mn);
-    l = l * a + w;
-    o0 = o0 * a + w * (float)vv[0];
-    o1 = o1 * a + w * (float)vv[1];
-    m = mn;
+
+  // Query rows past the last repeat it; they are not stored.
+  f16x8 qb[kQ][4];
+  const unsigned* mask_row[kQ];
+#pragma unroll
+  for (int u = 0; u < kQ; ++u) {
+    const int r = min(r0 + 16 * u + c, rows - 1), t = r / group;
+    const uint16_t* q = p.q + t * p.q_stride + (kh * group + r % group) * 128 + 8 * g;
+    mask_row[u] = reinterpret_cast<const unsigned*>(p.mask + (long long)t * words);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) qb[u][s] = *reinterpret_cast<const f16x8*>(q + 32 * s);
   }
-  so[wave][2 * lane] = o0;
-  so[wave][2 * lane + 1] = o1;
-  if (lane == 0) {
-    sm[wave] = m;
-    sl[wave] = l;
+
+  // A lane's offsets in a cache tile: K row c (+ 16), dims 32 s + 8 g; V row 4 g + i (+ 16),
+  // dims 8 c.  Bytes; 32 rows stay below 4 GiB where the tile is full.
+  const unsigned row_bytes = (unsigned)(p.row_stride * 2);
+  const unsigned k_off = (unsigned)c * row_bytes + 16u * g;
+  const unsigned v_off = (unsigned)(4 * g) * row_bytes + 16u * c;
+
+  auto load_k = [&](int tile, u32x4 (&k)[8]) {
+    if ((tile + 1) * kKeys <= p.prefix) {                  // a whole tile of the cache
+      const i32x4 rsrc = buffer_rsrc(p.k + kh * p.head_stride + (long long)tile * kKeys * p.row_stride, 0xffffffffu);
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          k[4 * a + s] = __builtin_bit_cast(u32x4, raw_buffer_load_b128(rsrc, (int)(k_off + 16u * a * row_bytes + 64u * s), 0, 0));
+      return;
+    }
+    const bool node = tile >= cache_tiles;
+    const int j0 = (node ? tile - cache_tiles : tile) * kKeys, n = node ? p.nodes : p.prefix;
+    const uint16_t* base = node ? p.kt + kh * p.thead_stride : p.k + kh * p.head_stride;
+    const long long stride = node ? p.trow_stride : p.row_stride;
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const int row = j0 + 16 * a + c;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        k[4 * a + s] = u32x4{0u, 0u, 0u, 0u};
+        if (row < n) k[4 * a + s] = *reinterpret_cast<const u32x4*>(base + row * stride + 32 * s + 8 * g);
+      }
+    }
+  };
+  auto load_v = [&](int tile, u32x4 (&v)[8]) {
+    if ((tile + 1) * kKeys <= p.prefix) {
+      const i32x4 rsrc = buffer_rsrc(p.v + kh * p.head_stride + (long long)tile * kKeys * p.row_stride, 0xffffffffu);
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[4 * a + i] = __builtin_bit_cast(u32x4, raw_buffer_load_b128(rsrc, (int)(v_off + (16u * a + i) * row_bytes), 0, 0));
+      return;
+    }
+    const bool node = tile >= cache_tiles;
+    const int j0 = (node ? tile - cache_tiles : tile) * kKeys, n = node ? p.nodes : p.prefix;
+    const uint16_t* base = node ? p.vt + kh * p.thead_stride : p.v + kh * p.head_stride;
+    const long long stride = node ? p.trow_stride : p.row_stride;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = j0 + 16 * a + 4 * g + i;
+        v[4 * a + i] = u32x4{0u, 0u, 0u, 0u};
+        if (row < n) v[4 * a + i] = *reinterpret_cast<const u32x4*>(base + row * stride + 8 * c);
+      }
+  };
+
+  float m[kQ];
+  f32x4 ls[kQ], o[kQ][8];
+#pragma unroll
+  for (int u = 0; u < kQ; ++u) {
+    m[u] = kNone;
+    ls[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[u][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  f16x8 ones;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ones[e] = (_Float16)1.0f;
+
+  const int step = p.splits * kW;
+  int tile = split * kW + wave;
+  u32x4 k[8], v[8];
+  if (tile < tiles) {
+    load_k(tile, k);
+    load_v(tile, v);
+  }
+  for (; tile < tiles; tile += step) {
+    const int next = tile + step;
+    f32x4 st[kQ][2];
+#pragma unroll
+    for (int u = 0; u < kQ; ++u)
+#pragma unroll
+      for (int a = 0; a < 2; ++a) st[u][a] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int u = 0; u < kQ; ++u)
+          st[u][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[4 * a + s]), qb[u][s], st[u][a], 0, 0, 0);
+    if (next < tiles) load_k(next, k);
+
+    const bool node = tile >= cache_tiles;
+    if ((tile + 1) * kKeys > p.prefix) {                   // the cache's last rows, or node rows
+#pragma unroll
+      for (int u = 0; u < kQ; ++u) {
+        const int n = p.prefix - tile * kKeys;             // cache rows in this tile
+        const int j = tile - cache_tiles, left = p.nodes - j * kKeys;
+        unsigned bits = node ? mask_row[u][j] : (1u << (n & 31)) - 1u;
+        if (node && left < kKeys) bits &= (1u << left) - 1u;
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) st[u][a][r] = (bits >> (16 * a + 4 * g + r)) & 1u ? st[u][a][r] : kNone;
+      }
+    }
+
+    // Each lane tests its own eight scores against the bound; only when some lane's pass it
+    // are maxima formed across the four lanes of a query.
+    float lm[kQ];
+    bool grow = false;
+#pragma unroll
+    for (int u = 0; u < kQ; ++u) {
+      lm[u] = fmaxf(fmaxf(fmaxf(st[u][0][0], st[u][0][1]), fmaxf(st[u][0][2], st[u][0][3])),
+                    fmaxf(fmaxf(st[u][1][0], st[u][1][1]), fmaxf(st[u][1][2], st[u][1][3])));
+      grow |= lm[u] * p.scale_log2 > m[u] + kLazy;         // -inf + kLazy is -inf: the first score grows it
+    }
+    if (__any(grow)) {
+#pragma unroll
+      for (int u = 0; u < kQ; ++u) {
+        float bm = fmaxf(lm[u], __shfl_xor(lm[u], 16));
+        bm = fmaxf(bm, __shfl_xor(bm, 32)) * p.scale_log2;
+        const float mn = bm > m[u] + kLazy ? bm : m[u];
+        const float alpha = mn == m[u] ? 1.0f : __builtin_amdgcn_exp2f(m[u] - mn);
+        ls[u] *= alpha;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[u][e] *= alpha;
+        m[u] = mn;
+      }
+    }
+    f16x8 pb[kQ];
+#pragma unroll
+    for (int u = 0; u < kQ; ++u) {
+      const float nref = m[u] == kNone ? 0.0f : -m[u];     // no row yet: every weight is 0
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        pb[u][e] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(st[u][e / 4][e % 4], p.scale_log2, nref));
+      ls[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pb[u], ls[u], 0, 0, 0);
+    }
+
+    // A weight of 0 keeps a finite V row out of a product, but not an infinity or a NaN: where
+    // a node tile holds one, such elements are taken out of the product and added, with the
+    // weights of the queries that see their row.
+    if (node && __any(any_nonfinite(v))) {
+      const int j0 = (tile - cache_tiles) * kKeys;
+      for (int j = 0; j < kKeys && j0 + j < p.nodes; ++j) {
+        const uint16_t* row = p.vt + kh * p.thead_stride + (j0 + j) * p.trow_stride + 32 * g;
+        const int slot = 4 * (j >> 4) + (j & 3), from = c + 16 * ((j & 15) >> 2);
+#pragma unroll
+        for (int u = 0; u < kQ; ++u) {
+          float w = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w = e == slot ? (float)pb[u][e] : w;
+          w = __shfl(w, from);
+          if ((mask_row[u][tile - cache_tiles] >> j) & 1u) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float x = (float)reinterpret_cast<const _Float16*>(row)[8 * i + e];
+                if (!(fabsf(x) < __builtin_inff())) o[u][e][i] = __builtin_fmaf(w, x, o[u][e][i]);
+              }
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const unsigned x = v[i][d];
+          if ((x & 0x7c00u) == 0x7c00u) v[i][d] &= 0xffff0000u;
+          if ((x & 0x7c000000u) == 0x7c000000u) v[i][d] &= 0x0000ffffu;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const f16x8 va = v_column(v, e);
+#pragma unroll
+      for (int u = 0; u < kQ; ++u) o[u][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[u], o[u][e], 0, 0, 0);
+    }
+    if (next < tiles) load_v(next, v);
+  }
+
+  // Fold the waves.
+#pragma unroll
+  for (int u = 0; u < kQ; ++u) {
+    float* dst = &fold_o[wave][16 * u + c][32 * g];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      *reinterpret_cast<f32x4*>(dst + 8 * i) = f32x4{o[u][0][i], o[u][1][i], o[u][2][i], o[u][3][i]};
+      *reinterpret_cast<f32x4*>(dst + 8 * i + 4) = f32x4{o[u][4][i], o[u][5][i], o[u][6][i], o[u][7][i]};
+    }
+    if (g == 0) {
+      fold_m[wave][16 * u + c] = m[u];
+      fold_l[wave][16 * u + c] = ls[u][0];
+    }
   }
   __syncthreads();
-  if (threadIdx.x < 128) {
-    float mx = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), acc = 0.0f, den = 0.0f;
-    for (int w = 0; w < 4; ++w) {
-      const float a = sm[w] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(sm[w] - mx);
-      acc += a * so[w][threadIdx.x];
-      den += a * sl[w];
+  // 16 threads per query row, 8 dims each.
+  for (int i = threadIdx.x; i < 16 * kQ * 16; i += kW * 64) {
+    const int q = i >> 4, d = 8 * (i & 15), r = r0 + q;
+    if (r >= rows) continue;
+    float mx = kNone, l = 0.0f, acc[8];
+#pragma unroll
+    for (int w = 0; w < kW; ++w) mx = fmaxf(mx, fold_m[w][q]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) {
+      const float mw = fold_m[w][q];
+      if (mw == kNone && fold_l[w][q] == 0.0f) continue;   // saw no row
+      const float a = mw == mx ? 1.0f : __builtin_amdgcn_exp2f(mw - mx);
+      l += a * fold_l[w][q];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += a * fold_o[w][q][d + e];
     }
-    reinterpret_cast<_Float16*>(p.out)[t * p.out_stride + h * 128 + threadIdx.x] =
-        to_f16(den > 0.0f || den != den ? acc / den : 0.0f);
+    if (p.splits == 1) {
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      f16x8 y;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = (_Float16)(l == 0.0f ? 0.0f : acc[e] * inv);
+      *reinterpret_cast<f16x8*>(p.out + (r / group) * p.out_stride + (kh * group + r % group) * 128 + d) = y;
+    } else {
+      const long long slot = ((long long)kh * rows + r) * p.splits + split;
+      float* dst = p.part_o + slot * 128 + d;
+      *reinterpret_cast<f32x4*>(dst) = f32x4{acc[0], acc[1], acc[2], acc[3]};
+      *reinterpret_cast<f32x4*>(dst + 4) = f32x4{acc[4], acc[5], acc[6], acc[7]};
+      if (d == 0) p.part_ml[slot] = float2{mx, l};
+    }
   }
+}
+
+// Folds the splits of one query row of one cache head: a wave, two dims per lane.
+__global__ __launch_bounds__(256) void tree_attention_merge_kernel(TreeAttnParams p) {
+  const int lane = threadIdx.x & 63;
+  const int group = p.heads / p.kv_heads, rows = p.nodes * group;
+  const int i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  if (i >= rows * p.kv_heads) return;
+  const float2* ml = p.part_ml + (long long)i * p.splits;
+  const float* po = p.part_o + (long long)i * p.splits * 128 + 2 * lane;
+  float mx = kNone;
+  for (int s = 0; s < p.splits; ++s) mx = fmaxf(mx, ml[s].x);
+  float l = 0.0f, a0 = 0.0f, a1 = 0.0f;
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 w = ml[s];
+    const float2 o = *reinterpret_cast<const float2*>(po + s * 128);
+    const float a = w.x == mx ? 1.0f : __builtin_amdgcn_exp2f(w.x - mx);
+    if (w.x == kNone && w.y == 0.0f) continue;             // saw no row
+    l += a * w.y;
+    a0 += a * o.x;
+    a1 += a * o.y;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int kh = i / rows, r = i % rows;
+  f16x2 y;
+  y[0] = (_Float16)(l == 0.0f ? 0.0f : a0 * inv);
+  y[1] = (_Float16)(l == 0.0f ? 0.0f : a1 * inv);
+  *reinterpret_cast<f16x2*>(p.out + (r / group) * p.out_stride + (kh * group + r % group) * 128 + 2 * lane) = y;
+}
+
+template <int kQ, int kW>
+hipError_t launch(const TreeAttnParams& p, int blocks, hipStream_t stream) {
+  hipLaunchKernelGGL((tree_attention_kernel<kQ, kW>), dim3(blocks * p.kv_heads * p.splits), dim3(kW * 64), 0, stream, p);
+  return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_tree_attention(const TreeAttnParams& p, hipStream_t stream) {
-  hipLaunchKernelGGL(tree_attention_kernel, dim3(p.nodes * p.heads), dim3(256), 0, stream, p);
+hipError_t launch_tree_attention(const TreeAttnParams& p, const TreeAttnPlan& plan, hipStream_t stream) {
+  hipError_t e;
+  switch (plan.q_tiles) {
+    case 1: e = launch<1, kTreeWaves1>(p, plan.blocks, stream); break;
+    case 2: e = launch<2, kTreeWaves2>(p, plan.blocks, stream); break;
+    default: e = launch<4, kTreeWaves4>(p, plan.blocks, stream); break;
+  }
+  if (e != hipSuccess || plan.splits == 1) return e;
+  const int rows = p.nodes * p.heads;
+  hipLaunchKernelGGL(tree_attention_merge_kernel, dim3((rows + 3) / 4), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
