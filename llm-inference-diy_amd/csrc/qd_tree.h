@@ -53,24 +53,24 @@ struct TreeAttnParams {
   float2* part_ml;          // [kv_heads][nodes * group][splits] (log2 reference, denominator)
 };
 
-// Launch plan: blocks of 16 * q_tiles query rows per cache head (a cache head's query rows
-// are its nodes x heads that share it), `splits` workgroups of `waves` waves for each.
+// Launch plan: blocks of block_rows query rows per cache head (a cache head's query rows are
+// its nodes x the heads that share it), `splits` workgroups of eight waves for each, of which
+// key_waves take different tiles of keys.
 struct TreeAttnPlan {
-  int q_tiles, waves, blocks, splits;
+  int block_rows, key_waves, blocks, splits;
 };
-constexpr int kTreeWaves1 = 8, kTreeWaves2 = 8, kTreeWaves4 = 4;
 
 // max_splits: what the workspace is sized for, at any prefix.
 inline TreeAttnPlan tree_attn_plan(int nodes, int heads, int kv_heads, int prefix, int num_cus, int* max_splits) {
   TreeAttnPlan plan;
   const int rows = nodes * (heads / kv_heads);
-  plan.q_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  plan.waves = plan.q_tiles == 1 ? kTreeWaves1 : plan.q_tiles == 2 ? kTreeWaves2 : kTreeWaves4;
-  plan.blocks = (rows + 16 * plan.q_tiles - 1) / (16 * plan.q_tiles);
+  plan.block_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  plan.key_waves = rows <= 32 ? 8 : rows <= 64 ? 4 : 2;
+  plan.blocks = (rows + plan.block_rows - 1) / plan.block_rows;
   const int most = num_cus / (plan.blocks * kv_heads);
   *max_splits = most < 1 ? 1 : most;
   const int tiles = (prefix + 31) / 32 + (nodes + 31) / 32;
-  const int by_tiles = (tiles + plan.waves - 1) / plan.waves;
+  const int by_tiles = (tiles + plan.key_waves - 1) / plan.key_waves;
   plan.splits = *max_splits < by_tiles ? *max_splits : by_tiles;
   return plan;
 }

@@ -60,20 +60,30 @@ __device__ __forceinline__ bool any_nonfinite(const u32x4 (&v)[8]) {
   return m[0] >= 0x7c00 || m[1] >= 0x7c00;
 }
 
-template <int kQ, int kW>
-__global__ __launch_bounds__(kW * 64) void tree_attention_kernel(TreeAttnParams p) {
-  __shared__ __align__(16) float fold_o[kW][16 * kQ][kFoldRow];
-  __shared__ float fold_m[kW][16 * kQ], fold_l[kW][16 * kQ];
+// A descriptor of wave-uniform values, held in scalar registers.
+__device__ __forceinline__ i32x4 wave_rsrc(const void* base, unsigned bytes) {
+  i32x4 r = buffer_rsrc(base, bytes);
+  r[0] = __builtin_amdgcn_readfirstlane(r[0]);
+  r[1] = __builtin_amdgcn_readfirstlane(r[1]);
+  r[2] = __builtin_amdgcn_readfirstlane(r[2]);
+  return r;
+}
+
+template <int kQ, int kQW, int kKW>
+__global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttnParams p) {
+  constexpr int kRows = 16 * kQ * kQW;                   // query rows of the block
+  constexpr int kThreads = kQW * kKW * 64;
+  __shared__ __align__(16) float fold_o[kKW][kRows][kFoldRow];
+  __shared__ float fold_m[kKW][kRows], fold_l[kKW][kRows];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int kw = wave / kQW, wq0 = 16 * kQ * (wave % kQW);   // key group, first row in the block
   const int c = lane & 15, g = lane >> 4;
   const int split = blockIdx.x % p.splits;
   const int kh = (blockIdx.x / p.splits) % p.kv_heads;
-  const int r0 = (blockIdx.x / p.splits / p.kv_heads) * 16 * kQ;   // the block's first query row
+  const int r0 = (blockIdx.x / p.splits / p.kv_heads) * kRows;   // the block's first query row
   const int group = p.heads / p.kv_heads;
   const int rows = p.nodes * group;
-  const int cache_tiles = (p.prefix + kKeys - 1) / kKeys;
-  const int tiles = cache_tiles + (p.nodes + kKeys - 1) / kKeys;
   const int words = (p.nodes + 63) / 64;
 
   // Query rows past the last repeat it; they are not stored.
@@ -81,66 +91,12 @@ __global__ __launch_bounds__(kW * 64) void tree_attention_kernel(TreeAttnParams 
   const unsigned* mask_row[kQ];
 #pragma unroll
   for (int u = 0; u < kQ; ++u) {
-    const int r = min(r0 + 16 * u + c, rows - 1), t = r / group;
+    const int r = min(r0 + wq0 + 16 * u + c, rows - 1), t = r / group;
     const uint16_t* q = p.q + t * p.q_stride + (kh * group + r % group) * 128 + 8 * g;
     mask_row[u] = reinterpret_cast<const unsigned*>(p.mask + (long long)t * words);
 #pragma unroll
     for (int s = 0; s < 4; ++s) qb[u][s] = *reinterpret_cast<const f16x8*>(q + 32 * s);
   }
-
-  // A lane's offsets in a cache tile: K row c (+ 16), dims 32 s + 8 g; V row 4 g + i (+ 16),
-  // dims 8 c.  Bytes; 32 rows stay below 4 GiB where the tile is full.
-  const unsigned row_bytes = (unsigned)(p.row_stride * 2);
-  const unsigned k_off = (unsigned)c * row_bytes + 16u * g;
-  const unsigned v_off = (unsigned)(4 * g) * row_bytes + 16u * c;
-
-  auto load_k = [&](int tile, u32x4 (&k)[8]) {
-    if ((tile + 1) * kKeys <= p.prefix) {                  // a whole tile of the cache
-      const i32x4 rsrc = buffer_rsrc(p.k + kh * p.head_stride + (long long)tile * kKeys * p.row_stride, 0xffffffffu);
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-          k[4 * a + s] = __builtin_bit_cast(u32x4, raw_buffer_load_b128(rsrc, (int)(k_off + 16u * a * row_bytes + 64u * s), 0, 0));
-      return;
-    }
-    const bool node = tile >= cache_tiles;
-    const int j0 = (node ? tile - cache_tiles : tile) * kKeys, n = node ? p.nodes : p.prefix;
-    const uint16_t* base = node ? p.kt + kh * p.thead_stride : p.k + kh * p.head_stride;
-    const long long stride = node ? p.trow_stride : p.row_stride;
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      const int row = j0 + 16 * a + c;
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        k[4 * a + s] = u32x4{0u, 0u, 0u, 0u};
-        if (row < n) k[4 * a + s] = *reinterpret_cast<const u32x4*>(base + row * stride + 32 * s + 8 * g);
-      }
-    }
-  };
-  auto load_v = [&](int tile, u32x4 (&v)[8]) {
-    if ((tile + 1) * kKeys <= p.prefix) {
-      const i32x4 rsrc = buffer_rsrc(p.v + kh * p.head_stride + (long long)tile * kKeys * p.row_stride, 0xffffffffu);
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          v[4 * a + i] = __builtin_bit_cast(u32x4, raw_buffer_load_b128(rsrc, (int)(v_off + (16u * a + i) * row_bytes), 0, 0));
-      return;
-    }
-    const bool node = tile >= cache_tiles;
-    const int j0 = (node ? tile - cache_tiles : tile) * kKeys, n = node ? p.nodes : p.prefix;
-    const uint16_t* base = node ? p.vt + kh * p.thead_stride : p.v + kh * p.head_stride;
-    const long long stride = node ? p.trow_stride : p.row_stride;
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = j0 + 16 * a + 4 * g + i;
-        v[4 * a + i] = u32x4{0u, 0u, 0u, 0u};
-        if (row < n) v[4 * a + i] = *reinterpret_cast<const u32x4*>(base + row * stride + 8 * c);
-      }
-  };
 
   float m[kQ];
   f32x4 ls[kQ], o[kQ][8];
@@ -155,16 +111,7 @@ __global__ __launch_bounds__(kW * 64) void tree_attention_kernel(TreeAttnParams 
 #pragma unroll
   for (int e = 0; e < 8; ++e) ones[e] = (_Float16)1.0f;
 
-  const int step = p.splits * kW;
-  int tile = split * kW + wave;
-  u32x4 k[8], v[8];
-  if (tile < tiles) {
-    load_k(tile, k);
-    load_v(tile, v);
-  }
-  for (; tile < tiles; tile += step) {
-    const int next = tile + step;
-    f32x4 st[kQ][2];
+  auto scores = [&](const u32x4 (&k)[8], f32x4 (&st)[kQ][2]) {
 #pragma unroll
     for (int u = 0; u < kQ; ++u)
 #pragma unroll
@@ -176,23 +123,9 @@ __global__ __launch_bounds__(kW * 64) void tree_attention_kernel(TreeAttnParams 
 #pragma unroll
         for (int u = 0; u < kQ; ++u)
           st[u][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[4 * a + s]), qb[u][s], st[u][a], 0, 0, 0);
-    if (next < tiles) load_k(next, k);
-
-    const bool node = tile >= cache_tiles;
-    if ((tile + 1) * kKeys > p.prefix) {                   // the cache's last rows, or node rows
-#pragma unroll
-      for (int u = 0; u < kQ; ++u) {
-        const int n = p.prefix - tile * kKeys;             // cache rows in this tile
-        const int j = tile - cache_tiles, left = p.nodes - j * kKeys;
-        unsigned bits = node ? mask_row[u][j] : (1u << (n & 31)) - 1u;
-        if (node && left < kKeys) bits &= (1u << left) - 1u;
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) st[u][a][r] = (bits >> (16 * a + 4 * g + r)) & 1u ? st[u][a][r] : kNone;
-      }
-    }
-
+  };
+  // Scores to weights; moves the reference maxima and scales the accumulators where needed.
+  auto weights = [&](const f32x4 (&st)[kQ][2], f16x8 (&pb)[kQ]) {
     // Each lane tests its own eight scores against the bound; only when some lane's pass it
     // are maxima formed across the four lanes of a query.
     float lm[kQ];
@@ -216,7 +149,6 @@ __global__ __launch_bounds__(kW * 64) void tree_attention_kernel(TreeAttnParams 
         m[u] = mn;
       }
     }
-    f16x8 pb[kQ];
 #pragma unroll
     for (int u = 0; u < kQ; ++u) {
       const float nref = m[u] == kNone ? 0.0f : -m[u];     // no row yet: every weight is 0
@@ -225,14 +157,67 @@ __global__ __launch_bounds__(kW * 64) void tree_attention_kernel(TreeAttnParams 
         pb[u][e] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(st[u][e / 4][e % 4], p.scale_log2, nref));
       ls[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pb[u], ls[u], 0, 0, 0);
     }
+  };
+  auto products = [&](const u32x4 (&v)[8], const f16x8 (&pb)[kQ]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const f16x8 va = v_column(v, e);
+#pragma unroll
+      for (int u = 0; u < kQ; ++u) o[u][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[u], o[u][e], 0, 0, 0);
+    }
+  };
 
+  // The tiles in the order that they are dealt out: the masked ones (node rows, and the
+  // cache's last rows if they do not fill a tile), then the cache's whole tiles.
+  const int full = p.prefix / kKeys, part = p.prefix % kKeys;
+  const int node_tiles = (p.nodes + kKeys - 1) / kKeys;
+  const int masked = node_tiles + (part ? 1 : 0);
+  const int step = p.splits * kKW;
+  int tile = r0 + wq0 < rows ? split * kKW + kw : full + masked;   // a wave without rows takes no tile
+  for (; tile < masked; tile += step) {
+    const bool node = tile < node_tiles;
+    const int j0 = kKeys * (node ? tile : full), n = node ? p.nodes : p.prefix;
+    const uint16_t* kb = node ? p.kt + kh * p.thead_stride : p.k + kh * p.head_stride;
+    const uint16_t* vb = node ? p.vt + kh * p.thead_stride : p.v + kh * p.head_stride;
+    const long long stride = node ? p.trow_stride : p.row_stride;
+    u32x4 k[8], v[8];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {                          // rows past the last are zeros
+      const int row = j0 + 16 * a + c;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        k[4 * a + s] = u32x4{0u, 0u, 0u, 0u};
+        if (row < n) k[4 * a + s] = *reinterpret_cast<const u32x4*>(kb + row * stride + 32 * s + 8 * g);
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = j0 + 16 * a + 4 * g + i;
+        v[4 * a + i] = u32x4{0u, 0u, 0u, 0u};
+        if (row < n) v[4 * a + i] = *reinterpret_cast<const u32x4*>(vb + row * stride + 8 * c);
+      }
+    f32x4 st[kQ][2];
+    scores(k, st);
+    unsigned bits[kQ];
+    const unsigned rows_here = n - j0 >= kKeys ? ~0u : (1u << (n - j0)) - 1u;
+#pragma unroll
+    for (int u = 0; u < kQ; ++u) {
+      bits[u] = (node ? mask_row[u][tile] : ~0u) & rows_here;
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st[u][a][r] = (bits[u] >> (16 * a + 4 * g + r)) & 1u ? st[u][a][r] : kNone;
+    }
+    f16x8 pb[kQ];
+    weights(st, pb);
     // A weight of 0 keeps a finite V row out of a product, but not an infinity or a NaN: where
-    // a node tile holds one, such elements are taken out of the product and added, with the
+    // the tile holds one, such elements are taken out of the product and added, with the
     // weights of the queries that see their row.
-    if (node && __any(any_nonfinite(v))) {
-      const int j0 = (tile - cache_tiles) * kKeys;
-      for (int j = 0; j < kKeys && j0 + j < p.nodes; ++j) {
-        const uint16_t* row = p.vt + kh * p.thead_stride + (j0 + j) * p.trow_stride + 32 * g;
+    if (__any(any_nonfinite(v))) {
+      for (int j = 0; j < kKeys && j0 + j < n; ++j) {
+        const _Float16* row = reinterpret_cast<const _Float16*>(vb + (j0 + j) * stride + 32 * g);
         const int slot = 4 * (j >> 4) + (j & 3), from = c + 16 * ((j & 15) >> 2);
 #pragma unroll
         for (int u = 0; u < kQ; ++u) {
@@ -240,12 +225,12 @@ __global__ __launch_bounds__(kW * 64) void tree_attention_kernel(TreeAttnParams 
 #pragma unroll
           for (int e = 0; e < 8; ++e) w = e == slot ? (float)pb[u][e] : w;
           w = __shfl(w, from);
-          if ((mask_row[u][tile - cache_tiles] >> j) & 1u) {
+          if ((bits[u] >> j) & 1u) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
-                const float x = (float)reinterpret_cast<const _Float16*>(row)[8 * i + e];
+                const float x = (float)row[8 * i + e];
                 if (!(fabsf(x) < __builtin_inff())) o[u][e][i] = __builtin_fmaf(w, x, o[u][e][i]);
               }
           }
@@ -260,41 +245,75 @@ __global__ __launch_bounds__(kW * 64) void tree_attention_kernel(TreeAttnParams 
           if ((x & 0x7c000000u) == 0x7c000000u) v[i][d] &= 0x0000ffffu;
         }
     }
+    products(v, pb);
+  }
+
+  // Whole tiles.  A lane's byte offsets in one (below 4 GiB: the cache is): K row c (+ 16),
+  // dims 32 s + 8 g; V row 4 g + i (+ 16), dims 8 c.  The next tile's K loads go out as soon as
+  // this one's are used, then its V loads; past the last tile the buffer is empty and the
+  // loads return zeros without reading, so the loop has no branch around a load and its waits
+  // count exactly the loads that it needs.
+  const unsigned row_bytes = (unsigned)(p.row_stride * 2);
+  const unsigned k_off = (unsigned)c * row_bytes + 16u * g;
+  const unsigned v_off = (unsigned)(4 * g) * row_bytes + 16u * c;
+  auto load_k = [&](int t, u32x4 (&k)[8]) {
+    const i32x4 rsrc = wave_rsrc(p.k + kh * p.head_stride + (long long)t * kKeys * p.row_stride, t < full ? 0xffffffffu : 0u);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const f16x8 va = v_column(v, e);
+    for (int a = 0; a < 2; ++a)
 #pragma unroll
-      for (int u = 0; u < kQ; ++u) o[u][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[u], o[u][e], 0, 0, 0);
+      for (int s = 0; s < 4; ++s)
+        k[4 * a + s] = __builtin_bit_cast(u32x4, raw_buffer_load_b128(rsrc, (int)(k_off + 16u * a * row_bytes + 64u * s), 0, 0));
+  };
+  auto load_v = [&](int t, u32x4 (&v)[8]) {
+    const i32x4 rsrc = wave_rsrc(p.v + kh * p.head_stride + (long long)t * kKeys * p.row_stride, t < full ? 0xffffffffu : 0u);
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[4 * a + i] = __builtin_bit_cast(u32x4, raw_buffer_load_b128(rsrc, (int)(v_off + (16u * a + i) * row_bytes), 0, 0));
+  };
+  tile -= masked;
+  if (tile < full) {
+    u32x4 k[8], v[8];
+    load_k(tile, k);
+    load_v(tile, v);
+    for (; tile < full; tile += step) {
+      f32x4 st[kQ][2];
+      f16x8 pb[kQ];
+      scores(k, st);
+      load_k(tile + step, k);
+      weights(st, pb);
+      products(v, pb);
+      load_v(tile + step, v);
     }
-    if (next < tiles) load_v(next, v);
   }
 
   // Fold the waves.
 #pragma unroll
   for (int u = 0; u < kQ; ++u) {
-    float* dst = &fold_o[wave][16 * u + c][32 * g];
+    float* dst = &fold_o[kw][wq0 + 16 * u + c][32 * g];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       *reinterpret_cast<f32x4*>(dst + 8 * i) = f32x4{o[u][0][i], o[u][1][i], o[u][2][i], o[u][3][i]};
       *reinterpret_cast<f32x4*>(dst + 8 * i + 4) = f32x4{o[u][4][i], o[u][5][i], o[u][6][i], o[u][7][i]};
     }
     if (g == 0) {
-      fold_m[wave][16 * u + c] = m[u];
-      fold_l[wave][16 * u + c] = ls[u][0];
+      fold_m[kw][wq0 + 16 * u + c] = m[u];
+      fold_l[kw][wq0 + 16 * u + c] = ls[u][0];
     }
   }
   __syncthreads();
   // 16 threads per query row, 8 dims each.
-  for (int i = threadIdx.x; i < 16 * kQ * 16; i += kW * 64) {
+  for (int i = threadIdx.x; i < kRows * 16; i += kThreads) {
     const int q = i >> 4, d = 8 * (i & 15), r = r0 + q;
     if (r >= rows) continue;
     float mx = kNone, l = 0.0f, acc[8];
 #pragma unroll
-    for (int w = 0; w < kW; ++w) mx = fmaxf(mx, fold_m[w][q]);
+    for (int w = 0; w < kKW; ++w) mx = fmaxf(mx, fold_m[w][q]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kW; ++w) {
+    for (int w = 0; w < kKW; ++w) {
       const float mw = fold_m[w][q];
       if (mw == kNone && fold_l[w][q] == 0.0f) continue;   // saw no row
       const float a = mw == mx ? 1.0f : __builtin_amdgcn_exp2f(mw - mx);
@@ -318,38 +337,61 @@ __global__ __launch_bounds__(kW * 64) void tree_attention_kernel(TreeAttnParams 
   }
 }
 
-// Folds the splits of one query row of one cache head: a wave, two dims per lane.
+// Folds the splits of one query row of one cache head: a wave, whose halves take every other
+// split, four dims per lane; eight splits' loads are in flight per half.
 __global__ __launch_bounds__(256) void tree_attention_merge_kernel(TreeAttnParams p) {
-  const int lane = threadIdx.x & 63;
+  constexpr int kBatch = 8;
+  const int lane = threadIdx.x & 63, half = lane >> 5, d = 4 * (lane & 31);
   const int group = p.heads / p.kv_heads, rows = p.nodes * group;
   const int i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   if (i >= rows * p.kv_heads) return;
   const float2* ml = p.part_ml + (long long)i * p.splits;
-  const float* po = p.part_o + (long long)i * p.splits * 128 + 2 * lane;
-  float mx = kNone;
-  for (int s = 0; s < p.splits; ++s) mx = fmaxf(mx, ml[s].x);
-  float l = 0.0f, a0 = 0.0f, a1 = 0.0f;
-#pragma unroll 4
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 w = ml[s];
-    const float2 o = *reinterpret_cast<const float2*>(po + s * 128);
-    const float a = w.x == mx ? 1.0f : __builtin_amdgcn_exp2f(w.x - mx);
-    if (w.x == kNone && w.y == 0.0f) continue;             // saw no row
-    l += a * w.y;
-    a0 += a * o.x;
-    a1 += a * o.y;
+  const float* po = p.part_o + (long long)i * p.splits * 128 + d;
+  float mx = kNone, l = 0.0f;
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s0 = half; s0 < p.splits; s0 += 2 * kBatch) {
+    float2 w[kBatch];
+    f32x4 x[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int s = min(s0 + 2 * j, p.splits - 1);
+      w[j] = ml[s];
+      x[j] = *reinterpret_cast<const f32x4*>(po + (long long)s * 128);
+      if (s0 + 2 * j >= p.splits) w[j] = float2{kNone, 0.0f};
+    }
+    float mn = mx;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) mn = fmaxf(mn, w[j].x);
+    const float keep = mn == mx ? 1.0f : __builtin_amdgcn_exp2f(mx - mn);
+    l *= keep;
+    acc *= keep;
+    mx = mn;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (w[j].x == kNone && w[j].y == 0.0f) continue;     // saw no row
+      const float a = w[j].x == mx ? 1.0f : __builtin_amdgcn_exp2f(w[j].x - mx);
+      l += a * w[j].y;
+      acc += a * x[j];
+    }
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float mo = __shfl_xor(mx, 32), mn = fmaxf(mx, mo);
+  const float a = mx == mn ? 1.0f : __builtin_amdgcn_exp2f(mx - mn), b = mo == mn ? 1.0f : __builtin_amdgcn_exp2f(mo - mn);
+  l = a * l + b * __shfl_xor(l, 32);
+  typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+  f16x4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float sum = a * acc[e] + b * __shfl_xor(acc[e], 32);
+    y[e] = (_Float16)(l == 0.0f ? 0.0f : sum / l);
+  }
   const int kh = i / rows, r = i % rows;
-  f16x2 y;
-  y[0] = (_Float16)(l == 0.0f ? 0.0f : a0 * inv);
-  y[1] = (_Float16)(l == 0.0f ? 0.0f : a1 * inv);
-  *reinterpret_cast<f16x2*>(p.out + (r / group) * p.out_stride + (kh * group + r % group) * 128 + 2 * lane) = y;
+  if (half == 0) *reinterpret_cast<f16x4*>(p.out + (r / group) * p.out_stride + (kh * group + r % group) * 128 + d) = y;
 }
 
-template <int kQ, int kW>
+template <int kQ, int kQW, int kKW>
 hipError_t launch(const TreeAttnParams& p, int blocks, hipStream_t stream) {
-  hipLaunchKernelGGL((tree_attention_kernel<kQ, kW>), dim3(blocks * p.kv_heads * p.splits), dim3(kW * 64), 0, stream, p);
+  hipLaunchKernelGGL((tree_attention_kernel<kQ, kQW, kKW>), dim3(blocks * p.kv_heads * p.splits), dim3(kQW * kKW * 64), 0,
+                     stream, p);
   return hipGetLastError();
 }
 
@@ -357,10 +399,11 @@ hipError_t launch(const TreeAttnParams& p, int blocks, hipStream_t stream) {
 
 hipError_t launch_tree_attention(const TreeAttnParams& p, const TreeAttnPlan& plan, hipStream_t stream) {
   hipError_t e;
-  switch (plan.q_tiles) {
-    case 1: e = launch<1, kTreeWaves1>(p, plan.blocks, stream); break;
-    case 2: e = launch<2, kTreeWaves2>(p, plan.blocks, stream); break;
-    default: e = launch<4, kTreeWaves4>(p, plan.blocks, stream); break;
+  switch (plan.block_rows) {
+    case 16: e = launch<1, 1, 8>(p, plan.blocks, stream); break;
+    case 32: e = launch<2, 1, 8>(p, plan.blocks, stream); break;
+    case 64: e = launch<2, 2, 4>(p, plan.blocks, stream); break;
+    default: e = launch<2, 4, 2>(p, plan.blocks, stream); break;
   }
   if (e != hipSuccess || plan.splits == 1) return e;
   const int rows = p.nodes * p.heads;
