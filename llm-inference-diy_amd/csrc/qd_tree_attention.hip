@@ -73,8 +73,10 @@ template <int kQ, int kQW, int kKW>
 __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttnParams p) {
   constexpr int kRows = 16 * kQ * kQW;                   // query rows of the block
   constexpr int kThreads = kQW * kKW * 64;
-  __shared__ __align__(16) float fold_o[kKW][kRows][kFoldRow];
-  __shared__ float fold_m[kKW][kRows], fold_l[kKW][kRows];
+  // K (and shared V) tiles during the scan, the waves' accumulators afterwards.
+  constexpr size_t kTiles = kQW == 1 ? (size_t)kKW * kKeys * 256 : (size_t)2 * kKW * kKeys * 512;
+  constexpr size_t kFold = (size_t)kKW * kRows * (kFoldRow + 2) * 4;
+  __shared__ __align__(16) char smem[kTiles > kFold ? kTiles : kFold];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int kw = wave / kQW, wq0 = 16 * kQ * (wave % kQW);   // key group, first row in the block
@@ -248,47 +250,128 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
     products(v, pb);
   }
 
-  // Whole tiles.  A lane's byte offsets in one (below 4 GiB: the cache is): K row c (+ 16),
-  // dims 32 s + 8 g; V row 4 g + i (+ 16), dims 8 c.  The next tile's K loads go out as soon as
-  // this one's are used, then its V loads; past the last tile the buffer is empty and the
-  // loads return zeros without reading, so the loop has no branch around a load and its waits
-  // count exactly the loads that it needs.
-  const unsigned row_bytes = (unsigned)(p.row_stride * 2);
-  const unsigned k_off = (unsigned)c * row_bytes + 16u * g;
-  const unsigned v_off = (unsigned)(4 * g) * row_bytes + 16u * c;
-  auto load_k = [&](int t, u32x4 (&k)[8]) {
-    const i32x4 rsrc = wave_rsrc(p.k + kh * p.head_stride + (long long)t * kKeys * p.row_stride, t < full ? 0xffffffffu : 0u);
+  // Whole tiles.  Loads read whole rows, four per instruction (instruction j: row 4 j + g,
+  // 16-byte chunk c of it); past the last tile the buffer is empty and they return zeros
+  // without reading, so the loops have no branch around a load and their waits count exactly
+  // the loads that they need.
+  const unsigned row_bytes = (unsigned)(p.row_stride * 2);   // 32 rows stay below 4 GiB where a tile is full
+  const unsigned off0 = (unsigned)g * row_bytes + 16u * c;
+  auto load = [&](const uint16_t* base, int t, int j) {
+    const i32x4 rsrc = wave_rsrc(base + kh * p.head_stride + (long long)t * kKeys * p.row_stride, t < full ? 0xffffffffu : 0u);
+    return __builtin_bit_cast(u32x4, raw_buffer_load_b128(rsrc, (int)(off0 + 4u * j * row_bytes), 0, 0));
+  };
+  // K rows in LDS: chunk q of row r at position q ^ (r % 16), so that neither the writes (whole
+  // rows) nor the operand reads (one chunk of 16 rows) meet on a bank.  V rows as they are.
+  auto put_k = [&](char* lk, int j, u32x4 x) {
+    const int r = 4 * j + g;
+    *reinterpret_cast<u32x4*>(lk + r * 256 + 16 * (c ^ (r & 15))) = x;
+  };
+  auto get_k = [&](const char* lk, u32x4 (&k)[8]) {
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int s = 0; s < 4; ++s)
-        k[4 * a + s] = __builtin_bit_cast(u32x4, raw_buffer_load_b128(rsrc, (int)(k_off + 16u * a * row_bytes + 64u * s), 0, 0));
-  };
-  auto load_v = [&](int t, u32x4 (&v)[8]) {
-    const i32x4 rsrc = wave_rsrc(p.v + kh * p.head_stride + (long long)t * kKeys * p.row_stride, t < full ? 0xffffffffu : 0u);
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[4 * a + i] = __builtin_bit_cast(u32x4, raw_buffer_load_b128(rsrc, (int)(v_off + (16u * a + i) * row_bytes), 0, 0));
+        k[4 * a + s] = *reinterpret_cast<const u32x4*>(lk + (16 * a + c) * 256 + 16 * ((4 * s + g) ^ c));
   };
   tile -= masked;
-  if (tile < full) {
-    u32x4 k[8], v[8];
-    load_k(tile, k);
-    load_v(tile, v);
-    for (; tile < full; tile += step) {
-      f32x4 st[kQ][2];
-      f16x8 pb[kQ];
-      scores(k, st);
-      load_k(tile + step, k);
-      weights(st, pb);
-      products(v, pb);
-      load_v(tile + step, v);
+  if constexpr (kQW == 1) {
+    // A wave's own tiles: K through its own LDS rows (in order within the wave, no barrier),
+    // V straight to registers: instruction 4 a + i of a lane is row 16 a + 4 g + i.
+    char* lk = smem + wave * kKeys * 256;
+    const unsigned voff = (unsigned)(4 * g) * row_bytes + 16u * c;
+    auto load_v = [&](int t, u32x4 (&v)[8]) {
+      const i32x4 rsrc = wave_rsrc(p.v + kh * p.head_stride + (long long)t * kKeys * p.row_stride, t < full ? 0xffffffffu : 0u);
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[4 * a + i] = __builtin_bit_cast(u32x4, raw_buffer_load_b128(rsrc, (int)(voff + (16u * a + i) * row_bytes), 0, 0));
+    };
+    if (tile < full) {
+      u32x4 kr[8], v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) kr[j] = load(p.k, tile, j);
+      load_v(tile, v);
+      for (; tile < full; tile += step) {
+        u32x4 k[8];
+        f32x4 st[kQ][2];
+        f16x8 pb[kQ];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) put_k(lk, j, kr[j]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) kr[j] = load(p.k, tile + step, j);
+        get_k(lk, k);
+        scores(k, st);
+        weights(st, pb);
+        products(v, pb);
+        load_v(tile + step, v);
+      }
+    }
+  } else {
+    // The key group's query waves share its tiles: each loads its part of the rows, two tiles
+    // ahead, and puts them into one of two LDS buffers; one barrier per tile (a buffer is
+    // written again only after the barrier behind its readers).  All key groups run the
+    // same number of rounds.
+    constexpr int kPart = 8 / kQW;
+    const int qw = wave % kQW;
+    int rounds = 0;
+    for (int w = 0; w < kKW; ++w) {
+      int t = split * kKW + w;
+      if (t < masked) t += (masked - t + step - 1) / step * step;
+      rounds = max(rounds, (full - (t - masked) + step - 1) / step);
+    }
+    const bool active = r0 + wq0 < rows;
+    if (!active) {                                         // loads and barriers only
+      tile = split * kKW + kw;
+      if (tile < masked) tile += (masked - tile + step - 1) / step * step;
+      tile -= masked;
+    }
+    u32x4 kr[2][kPart], vr[2][kPart];
+    auto fetch = [&](int t, u32x4 (&k)[kPart], u32x4 (&v)[kPart]) {
+#pragma unroll
+      for (int j = 0; j < kPart; ++j) k[j] = load(p.k, t, kPart * qw + j);
+#pragma unroll
+      for (int j = 0; j < kPart; ++j) v[j] = load(p.v, t, kPart * qw + j);
+    };
+    auto round = [&](int it, int buf, u32x4 (&kx)[kPart], u32x4 (&vx)[kPart]) {
+      char* lk = smem + (buf * kKW + kw) * kKeys * 512;
+      char* lv = lk + kKeys * 256;
+      const int t = tile + it * step;
+#pragma unroll
+      for (int j = 0; j < kPart; ++j) {
+        put_k(lk, kPart * qw + j, kx[j]);
+        *reinterpret_cast<u32x4*>(lv + (4 * (kPart * qw + j) + g) * 256 + 16 * c) = vx[j];
+      }
+      fetch(t + 2 * step, kx, vx);
+      __syncthreads();
+      if (active && t < full) {
+        u32x4 k[8], v[8];
+        f32x4 st[kQ][2];
+        f16x8 pb[kQ];
+        get_k(lk, k);
+        scores(k, st);
+        weights(st, pb);
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            v[4 * a + i] = *reinterpret_cast<const u32x4*>(lv + (16 * a + 4 * g + i) * 256 + 16 * c);
+        products(v, pb);
+      }
+    };
+    fetch(tile, kr[0], vr[0]);
+    fetch(tile + step, kr[1], vr[1]);
+    for (int it = 0; it < rounds; it += 2) {               // an odd count's last round finds no tile
+      round(it, 0, kr[0], vr[0]);
+      round(it + 1, 1, kr[1], vr[1]);
     }
   }
+  __syncthreads();                                         // LDS is taken over by the fold
 
   // Fold the waves.
+  float (*fold_o)[kRows][kFoldRow] = reinterpret_cast<float (*)[kRows][kFoldRow]>(smem);
+  float (*fold_m)[kRows] = reinterpret_cast<float (*)[kRows]>(smem + (size_t)kKW * kRows * kFoldRow * 4);
+  float (*fold_l)[kRows] = fold_m + kKW;
 #pragma unroll
   for (int u = 0; u < kQ; ++u) {
     float* dst = &fold_o[kw][wq0 + 16 * u + c][32 * g];
