@@ -212,7 +212,8 @@ int qd_tree_qkv_rope(qd_ctx* ctx, const uint16_t* qkv, long long qkv_stride, con
  * workspace: qd_tree_attention_workspace_bytes(ctx, nodes, num_heads) bytes of
  * device memory, 16-byte aligned; its contents need not survive between calls.
  * Requires 0 <= prefix <= max_seqlen; fp16 pointers 16-byte aligned, strides
- * multiples of 8; mask 8-byte aligned; out and workspace overlap neither each
+ * multiples of 8, tree_row_stride (and the context's
+ * kv_row_stride) at most 2^25; mask 8-byte aligned; out and workspace overlap neither each
  * other nor anything that is read (QD_EINVAL). */
 int qd_tree_attention(qd_ctx* ctx, const uint16_t* q, long long q_stride, const uint16_t* k_layer,
                       const uint16_t* v_layer, const uint16_t* k_tree, const uint16_t* v_tree,

@@ -23,6 +23,9 @@ bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0
 constexpr long long kMaxStride = 1LL << 40;
 bool stride_ok(long long s, long long least) { return s >= least && s % 8 == 0 && s <= kMaxStride; }
 
+// The attention addresses 32 rows by 32-bit byte offsets from the first of them.
+constexpr long long kMaxTreeRow = 1LL << 25;
+
 int check_device(const qd_ctx* ctx) {
   int dev = -1;
   if (hipGetDevice(&dev) != hipSuccess || dev != ctx->device)
@@ -155,8 +158,10 @@ int qd_tree_attention(qd_ctx* ctx, const uint16_t* q, long long q_stride, const 
   const long long row = (long long)num_heads * QD_HEAD_DIM;
   if (!stride_ok(q_stride, row) || !stride_ok(out_stride, row))
     return fail(QD_EINVAL, "q_stride and out_stride must be multiples of 8 and >= %lld", row);
-  if (!stride_ok(tree_row_stride, 8) || !stride_ok(tree_head_stride, 8))
-    return fail(QD_EINVAL, "tree strides must be positive multiples of 8 elements");
+  if (!stride_ok(tree_row_stride, 8) || !stride_ok(tree_head_stride, 8) || tree_row_stride > kMaxTreeRow)
+    return fail(QD_EINVAL, "tree strides must be positive multiples of 8 elements, rows at most 2^25 apart");
+  if (ctx->cfg.kv_row_stride > kMaxTreeRow)
+    return fail(QD_EINVAL, "the context's kv_row_stride %lld exceeds 2^25", ctx->cfg.kv_row_stride);
   const size_t need = qd_tree_attention_workspace_bytes(ctx, nodes, num_heads);
   if (workspace_bytes < need)
     return fail(QD_EINVAL, "workspace of %zu bytes is smaller than the %zu needed", workspace_bytes, need);

@@ -9,15 +9,15 @@
 // state each over all of the block's rows and are folded through LDS at the end.  Several
 // splits leave fp32 partials in the workspace, which a second launch folds.
 //
-// Nothing goes through LDS on the way to the products:
 //   S^T = K Q^T     (M = 16 keys, two tiles; N = 16 queries; K = 128 dims in four steps)
 //   O^T += V^T P^T  (M = 16 dims, eight tiles; N = 16 queries; K = 32 keys)
 // Operand lanes (c = l % 16, g = l / 16): A[c][8 g + e], B[8 g + e][c]; accumulator
-// D[4 g + r][c].  K rows feed A as loaded, 16 bytes a lane.  S^T leaves lane (g, c) the
-// scores of keys 16 a + 4 g + r of query c, which become P^T's B operand in place: its slot
-// 8 g + 4 a + r stands for key 16 a + 4 g + r.  V^T's A operand then needs, per dim, those
-// eight keys: a lane loads dims 8 c .. 8 c + 7 of its group's eight V rows (an instruction
-// reads four whole rows) and transposes the 8 x 8 halves with 32 byte permutations; the dims
+// D[4 g + r][c].  Loads take whole rows, four per instruction (16 bytes per lane, chunk c of
+// row 4 j + g): a K operand read straight from memory would touch a row per lane, which the
+// load path takes at one lane per clock.  K rows therefore go through LDS.  A lane's V rows
+// 4 j + g are P^T's operand slots as they are, when the K operands' rows are dealt so that
+// S^T leaves the lane the scores of the same eight keys; V^T's operand then is, per dim, the
+// lane's own eight rows, transposed by byte permutations (32 per 8 x 8 halves x 4).  The dims
 // tile e takes dim 8 c + e of every lane, so lane (g, c) ends with dims 32 g .. 32 g + 31 of
 // query c, and stores rows of its own.
 //
@@ -40,8 +40,12 @@ __device__ constexpr float kNone = -__builtin_inff();
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
-// Eight keys x eight dims of V as loaded, row 4 a + i of the group: va[e] slot 4 a + i is its
-// dim e.
+// What a lane holds of a V tile: dims 8 c .. 8 c + 7 of rows 4 j + g.
+struct Rows {
+  u32x4 x[8];
+};
+
+// Operand slot j: dim e of row j.
 __device__ __forceinline__ f16x8 v_column(const u32x4 (&v)[8], int e) {
   u32x4 r;
   const unsigned sel = e & 1 ? 0x07060302u : 0x05040100u;   // high or low halves of (second, first)
@@ -69,42 +73,54 @@ __device__ __forceinline__ i32x4 wave_rsrc(const void* base, unsigned bytes) {
   return r;
 }
 
+// Node of query row r (row = node * group + head of the group): exact for rows below 2^22 (the
+// reciprocal's estimate is off by at most one).
+__device__ __forceinline__ int row_node(int r, int group) {
+  int t = (int)((float)r * __builtin_amdgcn_rcpf((float)group));
+  if (t * group > r) --t;
+  if ((t + 1) * group <= r) ++t;
+  return t;
+}
+
 template <int kQ, int kQW, int kKW>
 __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttnParams p) {
   constexpr int kRows = 16 * kQ * kQW;                   // query rows of the block
   constexpr int kThreads = kQW * kKW * 64;
   // K (and shared V) tiles during the scan, the waves' accumulators afterwards.
   constexpr size_t kTiles = kQW == 1 ? (size_t)kKW * kKeys * 256 : (size_t)2 * kKW * kKeys * 512;
-  constexpr size_t kFold = (size_t)kKW * kRows * (kFoldRow + 2) * 4;
+  constexpr size_t kFold = (size_t)kKW * kRows * (kFoldRow + 2) * 4 + kQW * kKW * 4;
   __shared__ __align__(16) char smem[kTiles > kFold ? kTiles : kFold];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int kw = wave / kQW, wq0 = 16 * kQ * (wave % kQW);   // key group, first row in the block
   const int c = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x % p.splits;
-  const int kh = (blockIdx.x / p.splits) % p.kv_heads;
-  const int r0 = (blockIdx.x / p.splits / p.kv_heads) * kRows;   // the block's first query row
+  const int split = blockIdx.x, kh = blockIdx.y;
+  const int r0 = blockIdx.z * kRows;                     // the block's first query row
   const int group = p.heads / p.kv_heads;
   const int rows = p.nodes * group;
   const int words = (p.nodes + 63) / 64;
 
-  // Query rows past the last repeat it; they are not stored.
+  // Query rows past the last repeat it; they are not stored.  (Loaded before the first tiles: a
+  // wait for rows loaded later would hold up the tiles' loads in every round of the loop.)
   f16x8 qb[kQ][4];
   const unsigned* mask_row[kQ];
 #pragma unroll
   for (int u = 0; u < kQ; ++u) {
-    const int r = min(r0 + wq0 + 16 * u + c, rows - 1), t = r / group;
-    const uint16_t* q = p.q + t * p.q_stride + (kh * group + r % group) * 128 + 8 * g;
+    const int r = min(r0 + wq0 + 16 * u + c, rows - 1), t = row_node(r, group);
+    const uint16_t* q = p.q + t * p.q_stride + (kh * group + (r - t * group)) * 128 + 8 * g;
     mask_row[u] = reinterpret_cast<const unsigned*>(p.mask + (long long)t * words);
 #pragma unroll
     for (int s = 0; s < 4; ++s) qb[u][s] = *reinterpret_cast<const f16x8*>(q + 32 * s);
   }
 
-  float m[kQ];
+  // Per query, in log2 units: the reference maximum (0 while there is none), and the score that
+  // moves it (any score while there is none).
+  float m[kQ], lim[kQ];
   f32x4 ls[kQ], o[kQ][8];
 #pragma unroll
   for (int u = 0; u < kQ; ++u) {
-    m[u] = kNone;
+    m[u] = 0.0f;
+    lim[u] = kNone;
     ls[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[u][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -127,138 +143,80 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
           st[u][a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[4 * a + s]), qb[u][s], st[u][a], 0, 0, 0);
   };
   // Scores to weights; moves the reference maxima and scales the accumulators where needed.
-  auto weights = [&](const f32x4 (&st)[kQ][2], f16x8 (&pb)[kQ]) {
+  auto weights = [&](f32x4 (&st)[kQ][2], f16x8 (&pb)[kQ]) {
     // Each lane tests its own eight scores against the bound; only when some lane's pass it
-    // are maxima formed across the four lanes of a query.
+    // are maxima formed across the four lanes of a query.  (Scaled first: a maximum of values
+    // that were just computed needs no instruction to quiet NaN inputs.)
     float lm[kQ];
     bool grow = false;
 #pragma unroll
     for (int u = 0; u < kQ; ++u) {
+#pragma unroll
+      for (int a = 0; a < 2; ++a) st[u][a] *= p.scale_log2;
       lm[u] = fmaxf(fmaxf(fmaxf(st[u][0][0], st[u][0][1]), fmaxf(st[u][0][2], st[u][0][3])),
                     fmaxf(fmaxf(st[u][1][0], st[u][1][1]), fmaxf(st[u][1][2], st[u][1][3])));
-      grow |= lm[u] * p.scale_log2 > m[u] + kLazy;         // -inf + kLazy is -inf: the first score grows it
+      grow |= lm[u] > lim[u];
     }
     if (__any(grow)) {
 #pragma unroll
       for (int u = 0; u < kQ; ++u) {
         float bm = fmaxf(lm[u], __shfl_xor(lm[u], 16));
-        bm = fmaxf(bm, __shfl_xor(bm, 32)) * p.scale_log2;
-        const float mn = bm > m[u] + kLazy ? bm : m[u];
-        const float alpha = mn == m[u] ? 1.0f : __builtin_amdgcn_exp2f(m[u] - mn);
-        ls[u] *= alpha;
+        bm = fmaxf(bm, __shfl_xor(bm, 32));
+        if (bm > lim[u]) {
+          const float alpha = lim[u] == kNone ? 0.0f : __builtin_amdgcn_exp2f(m[u] - bm);
+          ls[u] *= alpha;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[u][e] *= alpha;
-        m[u] = mn;
+          for (int e = 0; e < 8; ++e) o[u][e] *= alpha;
+          m[u] = bm;
+          lim[u] = bm + kLazy;
+        }
       }
     }
 #pragma unroll
     for (int u = 0; u < kQ; ++u) {
-      const float nref = m[u] == kNone ? 0.0f : -m[u];     // no row yet: every weight is 0
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        pb[u][e] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(st[u][e / 4][e % 4], p.scale_log2, nref));
+      for (int e = 0; e < 8; ++e) pb[u][e] = (_Float16)__builtin_amdgcn_exp2f(st[u][e / 4][e % 4] - m[u]);
       ls[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pb[u], ls[u], 0, 0, 0);
     }
   };
-  auto products = [&](const u32x4 (&v)[8], const f16x8 (&pb)[kQ]) {
+  auto products = [&](const Rows& v, const f16x8 (&pb)[kQ]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const f16x8 va = v_column(v, e);
+      const f16x8 va = v_column(v.x, e);
 #pragma unroll
       for (int u = 0; u < kQ; ++u) o[u][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[u], o[u][e], 0, 0, 0);
     }
   };
 
-  // The tiles in the order that they are dealt out: the masked ones (node rows, and the
-  // cache's last rows if they do not fill a tile), then the cache's whole tiles.
-  const int full = p.prefix / kKeys, part = p.prefix % kKeys;
-  const int node_tiles = (p.nodes + kKeys - 1) / kKeys;
-  const int masked = node_tiles + (part ? 1 : 0);
-  const int step = p.splits * kKW;
-  int tile = r0 + wq0 < rows ? split * kKW + kw : full + masked;   // a wave without rows takes no tile
-  for (; tile < masked; tile += step) {
-    const bool node = tile < node_tiles;
-    const int j0 = kKeys * (node ? tile : full), n = node ? p.nodes : p.prefix;
-    const uint16_t* kb = node ? p.kt + kh * p.thead_stride : p.k + kh * p.head_stride;
-    const uint16_t* vb = node ? p.vt + kh * p.thead_stride : p.v + kh * p.head_stride;
-    const long long stride = node ? p.trow_stride : p.row_stride;
-    u32x4 k[8], v[8];
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {                          // rows past the last are zeros
-      const int row = j0 + 16 * a + c;
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        k[4 * a + s] = u32x4{0u, 0u, 0u, 0u};
-        if (row < n) k[4 * a + s] = *reinterpret_cast<const u32x4*>(kb + row * stride + 32 * s + 8 * g);
-      }
-    }
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = j0 + 16 * a + 4 * g + i;
-        v[4 * a + i] = u32x4{0u, 0u, 0u, 0u};
-        if (row < n) v[4 * a + i] = *reinterpret_cast<const u32x4*>(vb + row * stride + 8 * c);
-      }
-    f32x4 st[kQ][2];
-    scores(k, st);
-    unsigned bits[kQ];
-    const unsigned rows_here = n - j0 >= kKeys ? ~0u : (1u << (n - j0)) - 1u;
-#pragma unroll
-    for (int u = 0; u < kQ; ++u) {
-      bits[u] = (node ? mask_row[u][tile] : ~0u) & rows_here;
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) st[u][a][r] = (bits[u] >> (16 * a + 4 * g + r)) & 1u ? st[u][a][r] : kNone;
-    }
-    f16x8 pb[kQ];
-    weights(st, pb);
-    // A weight of 0 keeps a finite V row out of a product, but not an infinity or a NaN: where
-    // the tile holds one, such elements are taken out of the product and added, with the
-    // weights of the queries that see their row.
-    if (__any(any_nonfinite(v))) {
-      for (int j = 0; j < kKeys && j0 + j < n; ++j) {
-        const _Float16* row = reinterpret_cast<const _Float16*>(vb + (j0 + j) * stride + 32 * g);
-        const int slot = 4 * (j >> 4) + (j & 3), from = c + 16 * ((j & 15) >> 2);
-#pragma unroll
-        for (int u = 0; u < kQ; ++u) {
-          float w = 0.0f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) w = e == slot ? (float)pb[u][e] : w;
-          w = __shfl(w, from);
-          if ((bits[u] >> j) & 1u) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const float x = (float)row[8 * i + e];
-                if (!(fabsf(x) < __builtin_inff())) o[u][e][i] = __builtin_fmaf(w, x, o[u][e][i]);
-              }
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-          const unsigned x = v[i][d];
-          if ((x & 0x7c00u) == 0x7c00u) v[i][d] &= 0xffff0000u;
-          if ((x & 0x7c000000u) == 0x7c000000u) v[i][d] &= 0x0000ffffu;
-        }
-    }
-    products(v, pb);
-  }
-
-  // Whole tiles.  Loads read whole rows, four per instruction (instruction j: row 4 j + g,
-  // 16-byte chunk c of it); past the last tile the buffer is empty and they return zeros
-  // without reading, so the loops have no branch around a load and their waits count exactly
-  // the loads that they need.
-  const unsigned row_bytes = (unsigned)(p.row_stride * 2);   // 32 rows stay below 4 GiB where a tile is full
-  const unsigned off0 = (unsigned)g * row_bytes + 16u * c;
-  auto load = [&](const uint16_t* base, int t, int j) {
-    const i32x4 rsrc = wave_rsrc(base + kh * p.head_stride + (long long)t * kKeys * p.row_stride, t < full ? 0xffffffffu : 0u);
-    return __builtin_bit_cast(u32x4, raw_buffer_load_b128(rsrc, (int)(off0 + 4u * j * row_bytes), 0, 0));
+  // The tiles: the cache's rows, then the node rows, each in tiles of their own.  A load reads
+  // four whole rows: instruction j of a tile row 4 j + g, 16-byte chunk c of it.  A tile's descriptor
+  // ends with the last row that is there, so that rows past it (and tiles past the last) come as
+  // zeros without being read: the loops have no branch around a load, and their waits count
+  // exactly the loads that they need.
+  const int cache_tiles = (p.prefix + kKeys - 1) / kKeys;
+  const int tiles = cache_tiles + (p.nodes + kKeys - 1) / kKeys;
+  struct Source {
+    i32x4 k, v;
+    unsigned off, row4;
+  };
+  auto source = [&](int t) {
+    const bool node = t >= cache_tiles;
+    const int row = (node ? t - cache_tiles : t) * kKeys, left = (node ? p.nodes : p.prefix) - row;
+    const long long stride = node ? p.trow_stride : p.row_stride, head = kh * (node ? p.thead_stride : p.head_stride);
+    const unsigned row_bytes = (unsigned)(stride * 2);
+    const unsigned bytes = t >= tiles ? 0u : (unsigned)(min(left, kKeys) - 1) * row_bytes + 256u;
+    Source x;
+    x.k = wave_rsrc((node ? p.kt : p.k) + head + row * stride, bytes);
+    x.v = wave_rsrc((node ? p.vt : p.v) + head + row * stride, bytes);
+    x.off = (unsigned)g * row_bytes + 16u * c;
+    x.row4 = 4u * row_bytes;
+    return x;
+  };
+  auto load_k = [&](const Source& x, int j) {
+    return __builtin_bit_cast(u32x4, raw_buffer_load_b128(x.k, (int)(x.off + j * x.row4), 0, 0));
+  };
+  auto load_v = [&](const Source& x, int j) {
+    return __builtin_bit_cast(u32x4, raw_buffer_load_b128(x.v, (int)(x.off + j * x.row4), 0, 0));
   };
   // K rows in LDS: chunk q of row r at position q ^ (r % 16), so that neither the writes (whole
   // rows) nor the operand reads (one chunk of 16 rows) meet on a bank.  V rows as they are.
@@ -266,46 +224,81 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
     const int r = 4 * j + g;
     *reinterpret_cast<u32x4*>(lk + r * 256 + 16 * (c ^ (r & 15))) = x;
   };
+  // K operand a, row c: key 16 a + 4 (c % 4) + c / 4, so that the accumulator's row 4 g + r is
+  // key 4 (4 a + r) + g: the weights of a lane are those of the V rows that it loads.
+  const int krow = 4 * (c & 3) + (c >> 2);
   auto get_k = [&](const char* lk, u32x4 (&k)[8]) {
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int s = 0; s < 4; ++s)
-        k[4 * a + s] = *reinterpret_cast<const u32x4*>(lk + (16 * a + c) * 256 + 16 * ((4 * s + g) ^ c));
+        k[4 * a + s] = *reinterpret_cast<const u32x4*>(lk + (16 * a + krow) * 256 + 16 * ((4 * s + g) ^ krow));
   };
-  tile -= masked;
+  bool nonfinite = false;                                  // a node tile held infinities or NaN
+  // Scores, weights and products of one tile; `values` delivers the V rows when they are wanted.
+  auto tile_step = [&](int t, const char* lk, auto&& values) {
+    f32x4 st[kQ][2];
+    f16x8 pb[kQ];
+    {
+      u32x4 k[8];
+      get_k(lk, k);
+      scores(k, st);
+    }
+    const bool node = t >= cache_tiles;
+    if (node || (t + 1) * kKeys > p.prefix) {              // node rows, or the cache's last rows
+      const int n = node ? p.nodes - (t - cache_tiles) * kKeys : p.prefix - t * kKeys;
+      const unsigned rows_here = n >= kKeys ? ~0u : (1u << n) - 1u;
+#pragma unroll
+      for (int u = 0; u < kQ; ++u) {
+        const unsigned bits = ((node ? mask_row[u][t - cache_tiles] : ~0u) & rows_here) >> g;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) st[u][j / 4][j % 4] = (bits >> (4 * j)) & 1u ? st[u][j / 4][j % 4] : kNone;
+      }
+    }
+    weights(st, pb);
+    Rows v;
+    values(v);
+    // A weight of 0 keeps a finite V row out of a product, but not an infinity or a NaN: in a
+    // node tile such elements count as 0, and the fold adds them where they are seen.
+    if (node && __any(any_nonfinite(v.x))) {
+      nonfinite = true;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const unsigned x = v.x[i][d];
+          unsigned keep = (x & 0x7c00u) == 0x7c00u ? 0xffff0000u : 0xffffffffu;
+          if ((x & 0x7c000000u) == 0x7c000000u) keep &= 0x0000ffffu;
+          v.x[i][d] = x & keep;
+        }
+    }
+    products(v, pb);
+  };
+
+  const int step = p.splits * kKW;
+  int tile = split * kKW + kw;
   if constexpr (kQW == 1) {
     // A wave's own tiles: K through its own LDS rows (in order within the wave, no barrier),
-    // V straight to registers: instruction 4 a + i of a lane is row 16 a + 4 g + i.
+    // V straight to registers.
     char* lk = smem + wave * kKeys * 256;
-    const unsigned voff = (unsigned)(4 * g) * row_bytes + 16u * c;
-    auto load_v = [&](int t, u32x4 (&v)[8]) {
-      const i32x4 rsrc = wave_rsrc(p.v + kh * p.head_stride + (long long)t * kKeys * p.row_stride, t < full ? 0xffffffffu : 0u);
+    u32x4 kr[8];
+    Rows v;
+    {
+      const Source x = source(tile);
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+      for (int j = 0; j < 8; ++j) kr[j] = load_k(x, j);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          v[4 * a + i] = __builtin_bit_cast(u32x4, raw_buffer_load_b128(rsrc, (int)(voff + (16u * a + i) * row_bytes), 0, 0));
-    };
-    if (tile < full) {
-      u32x4 kr[8], v[8];
+      for (int j = 0; j < 8; ++j) v.x[j] = load_v(x, j);
+    }
+    for (; tile < tiles; tile += step) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) kr[j] = load(p.k, tile, j);
-      load_v(tile, v);
-      for (; tile < full; tile += step) {
-        u32x4 k[8];
-        f32x4 st[kQ][2];
-        f16x8 pb[kQ];
+      for (int j = 0; j < 8; ++j) put_k(lk, j, kr[j]);
+      const Source next = source(tile + step);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) put_k(lk, j, kr[j]);
+      for (int j = 0; j < 8; ++j) kr[j] = load_k(next, j);
+      tile_step(tile, lk, [&](Rows& x) { x = v; });
 #pragma unroll
-        for (int j = 0; j < 8; ++j) kr[j] = load(p.k, tile + step, j);
-        get_k(lk, k);
-        scores(k, st);
-        weights(st, pb);
-        products(v, pb);
-        load_v(tile + step, v);
-      }
+      for (int j = 0; j < 8; ++j) v.x[j] = load_v(next, j);
     }
   } else {
     // The key group's query waves share its tiles: each loads its part of the rows, two tiles
@@ -314,24 +307,15 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
     // same number of rounds.
     constexpr int kPart = 8 / kQW;
     const int qw = wave % kQW;
-    int rounds = 0;
-    for (int w = 0; w < kKW; ++w) {
-      int t = split * kKW + w;
-      if (t < masked) t += (masked - t + step - 1) / step * step;
-      rounds = max(rounds, (full - (t - masked) + step - 1) / step);
-    }
+    const int rounds = (tiles - split * kKW + step - 1) / step;
     const bool active = r0 + wq0 < rows;
-    if (!active) {                                         // loads and barriers only
-      tile = split * kKW + kw;
-      if (tile < masked) tile += (masked - tile + step - 1) / step * step;
-      tile -= masked;
-    }
     u32x4 kr[2][kPart], vr[2][kPart];
     auto fetch = [&](int t, u32x4 (&k)[kPart], u32x4 (&v)[kPart]) {
+      const Source x = source(t);
 #pragma unroll
-      for (int j = 0; j < kPart; ++j) k[j] = load(p.k, t, kPart * qw + j);
+      for (int j = 0; j < kPart; ++j) k[j] = load_k(x, kPart * qw + j);
 #pragma unroll
-      for (int j = 0; j < kPart; ++j) v[j] = load(p.v, t, kPart * qw + j);
+      for (int j = 0; j < kPart; ++j) v[j] = load_v(x, kPart * qw + j);
     };
     auto round = [&](int it, int buf, u32x4 (&kx)[kPart], u32x4 (&vx)[kPart]) {
       char* lk = smem + (buf * kKW + kw) * kKeys * 512;
@@ -344,20 +328,11 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
       }
       fetch(t + 2 * step, kx, vx);
       __syncthreads();
-      if (active && t < full) {
-        u32x4 k[8], v[8];
-        f32x4 st[kQ][2];
-        f16x8 pb[kQ];
-        get_k(lk, k);
-        scores(k, st);
-        weights(st, pb);
+      if (active && t < tiles)
+        tile_step(t, lk, [&](Rows& v) {
 #pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            v[4 * a + i] = *reinterpret_cast<const u32x4*>(lv + (16 * a + 4 * g + i) * 256 + 16 * c);
-        products(v, pb);
-      }
+          for (int j = 0; j < 8; ++j) v.x[j] = *reinterpret_cast<const u32x4*>(lv + (4 * j + g) * 256 + 16 * c);
+        });
     };
     fetch(tile, kr[0], vr[0]);
     fetch(tile + step, kr[1], vr[1]);
@@ -372,6 +347,8 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
   float (*fold_o)[kRows][kFoldRow] = reinterpret_cast<float (*)[kRows][kFoldRow]>(smem);
   float (*fold_m)[kRows] = reinterpret_cast<float (*)[kRows]>(smem + (size_t)kKW * kRows * kFoldRow * 4);
   float (*fold_l)[kRows] = fold_m + kKW;
+  int* fold_bad = reinterpret_cast<int*>(fold_l + kKW);
+  if (lane == 0) fold_bad[wave] = nonfinite;
 #pragma unroll
   for (int u = 0; u < kQ; ++u) {
     float* dst = &fold_o[kw][wq0 + 16 * u + c][32 * g];
@@ -381,7 +358,7 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
       *reinterpret_cast<f32x4*>(dst + 8 * i + 4) = f32x4{o[u][4][i], o[u][5][i], o[u][6][i], o[u][7][i]};
     }
     if (g == 0) {
-      fold_m[kw][wq0 + 16 * u + c] = m[u];
+      fold_m[kw][wq0 + 16 * u + c] = lim[u] == kNone ? kNone : m[u];
       fold_l[kw][wq0 + 16 * u + c] = ls[u][0];
     }
   }
@@ -389,7 +366,9 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
   // 16 threads per query row, 8 dims each.
   for (int i = threadIdx.x; i < kRows * 16; i += kThreads) {
     const int q = i >> 4, d = 8 * (i & 15), r = r0 + q;
-    if (r >= rows) continue;
+    if (r >= rows) break;
+    const int t = row_node(r, group);
+    uint16_t* out = p.out + t * p.out_stride + (kh * group + (r - t * group)) * 128 + d;
     float mx = kNone, l = 0.0f, acc[8];
 #pragma unroll
     for (int w = 0; w < kKW; ++w) mx = fmaxf(mx, fold_m[w][q]);
@@ -404,12 +383,24 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
 #pragma unroll
       for (int e = 0; e < 8; ++e) acc[e] += a * fold_o[w][q][d + e];
     }
+    bool bad = false;
+    for (int w = 0; w < kQW * kKW; ++w) bad |= fold_bad[w] != 0;
+    if (bad) {                                             // infinities and NaN of this workgroup's node tiles
+      const uint64_t* mask = p.mask + (long long)t * words;
+      for (int j = 0; j < p.nodes; ++j) {
+        if ((cache_tiles + j / kKeys) % step / kKW != split || !((mask[j >> 6] >> (j & 63)) & 1u)) continue;
+        const f16x8 x = *reinterpret_cast<const f16x8*>(p.vt + kh * p.thead_stride + j * p.trow_stride + d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (!(fabsf((float)x[e]) < __builtin_inff())) acc[e] += (float)x[e];
+      }
+    }
     if (p.splits == 1) {
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       f16x8 y;
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = (_Float16)(l == 0.0f ? 0.0f : acc[e] * inv);
-      *reinterpret_cast<f16x8*>(p.out + (r / group) * p.out_stride + (kh * group + r % group) * 128 + d) = y;
+      *reinterpret_cast<f16x8*>(out) = y;
     } else {
       const long long slot = ((long long)kh * rows + r) * p.splits + split;
       float* dst = p.part_o + slot * 128 + d;
@@ -473,7 +464,7 @@ __global__ __launch_bounds__(256) void tree_attention_merge_kernel(TreeAttnParam
 
 template <int kQ, int kQW, int kKW>
 hipError_t launch(const TreeAttnParams& p, int blocks, hipStream_t stream) {
-  hipLaunchKernelGGL((tree_attention_kernel<kQ, kQW, kKW>), dim3(blocks * p.kv_heads * p.splits), dim3(kQW * kKW * 64), 0,
+  hipLaunchKernelGGL((tree_attention_kernel<kQ, kQW, kKW>), dim3(p.splits, p.kv_heads, blocks), dim3(kQW * kKW * 64), 0,
                      stream, p);
   return hipGetLastError();
 }

@@ -276,9 +276,9 @@ def test_rows_of_the_cache_itself_as_node_rows(qdiy):
 
 
 def test_offsets_past_32_bits(qdiy):
-    """Node rows 2^27 elements apart: row 20 starts past 4 GiB.  (A cache is held below 4 GiB by
-    its context.)"""
-    T, row = 21, 1 << 27
+    """Node rows 2^25 elements apart, the most that the call takes: row 64 starts at 4 GiB.  (A
+    cache is held below 4 GiB by its context.)"""
+    T, row = 70, 1 << 25
     c = Case(qdiy, 1, 1, 40, T, seed=41)
     big = torch.zeros((T - 1) * row + D, dtype=torch.float16, device="cuda")
     want = c.result().copy()
@@ -307,7 +307,7 @@ def test_refusals(qdiy):
 
     bad = [dict(T=0), dict(T=1025), dict(P=-1), dict(P=24), dict(H=0), dict(H=6), dict(H=8192), dict(hd=64),
            dict(qs=8 * D - 8), dict(qs=8 * D + 4), dict(os=8 * D - 8), dict(os=8 * D + 2), dict(trow=0),
-           dict(trow=12), dict(thead=-8), dict(thead=1 << 41), dict(wsb=c.ws.numel() - 1),
+           dict(trow=12), dict(trow=(1 << 25) + 8), dict(thead=-8), dict(thead=1 << 41), dict(wsb=c.ws.numel() - 1),
            dict(mask=good["mask"] + 4), dict(ws=good["ws"] + 8)]
     bad += [{n: None} for n in ("q", "k", "v", "kt", "vt", "mask", "out", "ws")]
     bad += [{n: good[n] + 8} for n in ("q", "k", "v", "kt", "vt", "out")]
