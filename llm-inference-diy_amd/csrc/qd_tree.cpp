@@ -136,8 +136,8 @@ int qd_tree_qkv_rope(qd_ctx* ctx, const uint16_t* qkv, long long qkv_stride, con
 size_t qd_tree_attention_workspace_bytes(const qd_ctx* ctx, int nodes, int num_heads) {
   if (check_shape(ctx, 0, nodes) != QD_OK || check_heads(ctx, num_heads, QD_HEAD_DIM) != QD_OK) return 0;
   int splits = 1;
-  (void)qd::tree_attn_plan(nodes, num_heads, ctx->cfg.num_heads, 0, ctx->num_cus, &splits);
-  return (size_t)nodes * num_heads * splits * (128 + 2) * sizeof(float);
+  const qd::TreeAttnPlan plan = qd::tree_attn_plan(nodes, num_heads, ctx->cfg.num_heads, 0, ctx->num_cus, &splits);
+  return (size_t)plan.blocks * ctx->cfg.num_heads * splits * plan.block_rows * (128 + 2) * sizeof(float);
 }
 
 int qd_tree_attention(qd_ctx* ctx, const uint16_t* q, long long q_stride, const uint16_t* k_layer,
@@ -177,11 +177,11 @@ int qd_tree_attention(qd_ctx* ctx, const uint16_t* q, long long q_stride, const 
   int max_splits = 1;
   const qd::TreeAttnPlan plan = qd::tree_attn_plan(nodes, num_heads, kvh, prefix, ctx->num_cus, &max_splits);
   float* part_o = static_cast<float*>(workspace);
-  float2* part_ml = reinterpret_cast<float2*>(part_o + (size_t)nodes * num_heads * max_splits * 128);
+  float2* part_ml = reinterpret_cast<float2*>(part_o + (size_t)plan.blocks * kvh * max_splits * plan.block_rows * 128);
   const qd::TreeAttnParams p{q, k_layer, v_layer, k_tree, v_tree, mask, out, q_stride, out_stride,
                              ctx->cfg.kv_row_stride, ctx->cfg.kv_head_stride, tree_row_stride, tree_head_stride,
                              prefix, nodes, num_heads, kvh, (float)(1.4426950408889634 / std::sqrt(128.0)),
-                             plan.splits, part_o, part_ml};
+                             plan.splits, reinterpret_cast<decltype(qd::TreeAttnParams::part_o)>(part_o), part_ml};
   const hipError_t e = qd::launch_tree_attention(p, plan, stream);
   return e == hipSuccess ? QD_OK : hip_fail(e, "tree attention launch");
 }

@@ -49,8 +49,10 @@ struct TreeAttnParams {
   int prefix, nodes, heads, kv_heads;
   float scale_log2;         // log2(e) / sqrt(128)
   int splits;               // workgroups per block of query rows (TreeAttnPlan)
-  float* part_o;            // [kv_heads][nodes * group][splits][128], when splits > 1
-  float2* part_ml;          // [kv_heads][nodes * group][splits] (log2 reference, denominator)
+  // Partials, when splits > 1, per (block, cache head, split): the block's accumulators as
+  // fragments [block_rows / 16][8][64 lanes], and its rows' (log2 reference, denominator).
+  float __attribute__((ext_vector_type(4)))* part_o;
+  float2* part_ml;
 };
 
 // Launch plan: blocks of block_rows query rows per cache head (a cache head's query rows are

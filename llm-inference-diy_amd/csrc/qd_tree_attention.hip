@@ -34,7 +34,7 @@ namespace {
 
 constexpr int kKeys = 32;
 constexpr float kLazy = 8.0f;            // log2 of the largest softmax weight before a rescale
-constexpr int kFoldRow = 132;            // floats of a query's O row in LDS: 128, and 4 to spread the banks
+constexpr int kOutRow = 136;             // halves of an output row in LDS: 128, and 8 to spread the banks
 __device__ constexpr float kNone = -__builtin_inff();
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
   constexpr int kThreads = kQW * kKW * 64;
   // K (and shared V) tiles during the scan, the waves' accumulators afterwards.
   constexpr size_t kTiles = kQW == 1 ? (size_t)kKW * kKeys * 256 : (size_t)2 * kKW * kKeys * 512;
-  constexpr size_t kFold = (size_t)kKW * kRows * (kFoldRow + 2) * 4 + kQW * kKW * 4;
+  constexpr size_t kFold = (size_t)kKW * kRows * (128 * 4 + 8) + kQW * kKW * 4;
   __shared__ __align__(16) char smem[kTiles > kFold ? kTiles : kFold];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -341,125 +341,134 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
       round(it + 1, 1, kr[1], vr[1]);
     }
   }
-  __syncthreads();                                         // LDS is taken over by the fold
-
-  // Fold the waves.
-  float (*fold_o)[kRows][kFoldRow] = reinterpret_cast<float (*)[kRows][kFoldRow]>(smem);
-  float (*fold_m)[kRows] = reinterpret_cast<float (*)[kRows]>(smem + (size_t)kKW * kRows * kFoldRow * 4);
-  float (*fold_l)[kRows] = fold_m + kKW;
-  int* fold_bad = reinterpret_cast<int*>(fold_l + kKW);
-  if (lane == 0) fold_bad[wave] = nonfinite;
+  // Fold the key waves.  Every wave leaves its accumulators in LDS as they lie in its registers
+  // (fragment (u, e): 16 bytes of each lane); then each wave folds its share of the fragments
+  // and, of several splits, writes them out the same way.
+  __syncthreads();                                         // the tiles' LDS is taken over
+  constexpr int kWaves = kQW * kKW, kFrags = kQW * kQ * 8;
+  f32x4* frag = reinterpret_cast<f32x4*>(smem);            // [kKW][kFrags][64]
+  float2* state = reinterpret_cast<float2*>(frag + kKW * kFrags * 64);   // [kKW][kRows]
+  int* bad = reinterpret_cast<int*>(state + kKW * kRows);  // [kWaves]
 #pragma unroll
   for (int u = 0; u < kQ; ++u) {
-    float* dst = &fold_o[kw][wq0 + 16 * u + c][32 * g];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      *reinterpret_cast<f32x4*>(dst + 8 * i) = f32x4{o[u][0][i], o[u][1][i], o[u][2][i], o[u][3][i]};
-      *reinterpret_cast<f32x4*>(dst + 8 * i + 4) = f32x4{o[u][4][i], o[u][5][i], o[u][6][i], o[u][7][i]};
-    }
-    if (g == 0) {
-      fold_m[kw][wq0 + 16 * u + c] = lim[u] == kNone ? kNone : m[u];
-      fold_l[kw][wq0 + 16 * u + c] = ls[u][0];
-    }
+    for (int e = 0; e < 8; ++e) frag[(kw * kFrags + (wave % kQW * kQ + u) * 8 + e) * 64 + lane] = o[u][e];
+    if (g == 0) state[kw * kRows + wq0 + 16 * u + c] = float2{lim[u] == kNone ? kNone : m[u], ls[u][0]};
   }
+  if (lane == 0) bad[wave] = nonfinite;
   __syncthreads();
-  // 16 threads per query row, 8 dims each.
-  for (int i = threadIdx.x; i < kRows * 16; i += kThreads) {
-    const int q = i >> 4, d = 8 * (i & 15), r = r0 + q;
-    if (r >= rows) break;
-    const int t = row_node(r, group);
-    uint16_t* out = p.out + t * p.out_stride + (kh * group + (r - t * group)) * 128 + d;
-    float mx = kNone, l = 0.0f, acc[8];
+  bool any_bad = false;
 #pragma unroll
-    for (int w = 0; w < kKW; ++w) mx = fmaxf(mx, fold_m[w][q]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
+  for (int w = 0; w < kWaves; ++w) any_bad |= bad[w] != 0;
+  const int slot = (blockIdx.z * p.kv_heads + kh) * p.splits + split;
+  for (int f = wave; f < kFrags; f += kWaves) {
+    const int e = f & 7, q = 16 * (f >> 3) + c;            // the lane's row in the block
+    float mx = kNone, l = 0.0f;
+    float2 ml[kKW];
 #pragma unroll
     for (int w = 0; w < kKW; ++w) {
-      const float mw = fold_m[w][q];
-      if (mw == kNone && fold_l[w][q] == 0.0f) continue;   // saw no row
-      const float a = mw == mx ? 1.0f : __builtin_amdgcn_exp2f(mw - mx);
-      l += a * fold_l[w][q];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] += a * fold_o[w][q][d + e];
+      ml[w] = state[w * kRows + q];
+      mx = fmaxf(mx, ml[w].x);
     }
-    bool bad = false;
-    for (int w = 0; w < kQW * kKW; ++w) bad |= fold_bad[w] != 0;
-    if (bad) {                                             // infinities and NaN of this workgroup's node tiles
-      const uint64_t* mask = p.mask + (long long)t * words;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kKW; ++w) {
+      const float a = ml[w].x == mx ? 1.0f : __builtin_amdgcn_exp2f(ml[w].x - mx);   // -inf: saw no row
+      l += a * ml[w].y;
+      acc += a * frag[(w * kFrags + f) * 64 + lane];
+    }
+    const int r = min(r0 + q, rows - 1);
+    if (any_bad) {                                         // infinities and NaN of this workgroup's node tiles
+      const uint64_t* mask = p.mask + (long long)row_node(r, group) * words;
       for (int j = 0; j < p.nodes; ++j) {
         if ((cache_tiles + j / kKeys) % step / kKW != split || !((mask[j >> 6] >> (j & 63)) & 1u)) continue;
-        const f16x8 x = *reinterpret_cast<const f16x8*>(p.vt + kh * p.thead_stride + j * p.trow_stride + d);
+        const uint16_t* v = p.vt + kh * p.thead_stride + j * p.trow_stride + 32 * g + e;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (!(fabsf((float)x[e]) < __builtin_inff())) acc[e] += (float)x[e];
+        for (int i = 0; i < 4; ++i) {
+          const float x = (float)*reinterpret_cast<const _Float16*>(v + 8 * i);
+          if (!(fabsf(x) < __builtin_inff())) acc[i] += x;
+        }
       }
     }
-    if (p.splits == 1) {
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      f16x8 y;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = (_Float16)(l == 0.0f ? 0.0f : acc[e] * inv);
-      *reinterpret_cast<f16x8*>(out) = y;
+    if (p.splits > 1) {
+      if (r0 + q < rows) {
+        p.part_o[((long long)slot * kFrags + f) * 64 + lane] = acc;
+        if (e == 0 && g == 0) p.part_ml[(long long)slot * kRows + q] = float2{mx, l};
+      }
     } else {
-      const long long slot = ((long long)kh * rows + r) * p.splits + split;
-      float* dst = p.part_o + slot * 128 + d;
-      *reinterpret_cast<f32x4*>(dst) = f32x4{acc[0], acc[1], acc[2], acc[3]};
-      *reinterpret_cast<f32x4*>(dst + 4) = f32x4{acc[4], acc[5], acc[6], acc[7]};
-      if (d == 0) p.part_ml[slot] = float2{mx, l};
+      frag[f * 64 + lane] = l == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc / l;   // read by this wave alone
     }
+  }
+  if (p.splits > 1) return;
+  __syncthreads();
+  const float* folded = reinterpret_cast<const float*>(frag);
+  for (int i = threadIdx.x; i < kRows * 16; i += kThreads) {
+    const int q = i >> 4, d = 8 * (i & 15), r = r0 + q;    // dims d + e: fragment e, group d / 32, element d / 8 % 4
+    if (r >= rows) break;
+    f16x8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (_Float16)folded[(((q >> 4) * 8 + e) * 64 + 16 * (d >> 5) + (q & 15)) * 4 + ((d >> 3) & 3)];
+    const int t = row_node(r, group);
+    *reinterpret_cast<f16x8*>(p.out + t * p.out_stride + (kh * group + (r - t * group)) * 128 + d) = y;
   }
 }
 
-// Folds the splits of one query row of one cache head: a wave, whose halves take every other
-// split, four dims per lane; eight splits' loads are in flight per half.
-__global__ __launch_bounds__(256) void tree_attention_merge_kernel(TreeAttnParams p) {
-  constexpr int kBatch = 8;
-  const int lane = threadIdx.x & 63, half = lane >> 5, d = 4 * (lane & 31);
+// Folds the splits of 16 query rows of one cache head: a wave per fragment e, all of its splits'
+// loads of a batch in flight.
+__global__ __launch_bounds__(512) void tree_attention_merge_kernel(TreeAttnParams p, int block_rows) {
+  __shared__ __align__(16) _Float16 rows_out[16 * kOutRow];
+  constexpr int kBatch = 16;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int e = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int tiles = block_rows / 16, tile = blockIdx.x % tiles, block = blockIdx.x / tiles, kh = blockIdx.y;
   const int group = p.heads / p.kv_heads, rows = p.nodes * group;
-  const int i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  if (i >= rows * p.kv_heads) return;
-  const float2* ml = p.part_ml + (long long)i * p.splits;
-  const float* po = p.part_o + (long long)i * p.splits * 128 + d;
+  const int r0 = block * block_rows + 16 * tile;
+  if (r0 >= rows) return;
+  const long long slot = (long long)(block * p.kv_heads + kh) * p.splits;
+  const f32x4* po = p.part_o + ((slot * tiles + tile) * 8 + e) * 64 + lane;   // splits tiles * 8 * 64 apart
+  const float2* ml = p.part_ml + slot * block_rows + 16 * tile + c;
   float mx = kNone, l = 0.0f;
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s0 = half; s0 < p.splits; s0 += 2 * kBatch) {
+  for (int s0 = 0; s0 < p.splits; s0 += kBatch) {
     float2 w[kBatch];
     f32x4 x[kBatch];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      const int s = min(s0 + 2 * j, p.splits - 1);
-      w[j] = ml[s];
-      x[j] = *reinterpret_cast<const f32x4*>(po + (long long)s * 128);
-      if (s0 + 2 * j >= p.splits) w[j] = float2{kNone, 0.0f};
+      const int s = min(s0 + j, p.splits - 1);
+      w[j] = ml[(long long)s * block_rows];                // rows that are not there: whatever the workspace holds,
+      x[j] = po[(long long)s * tiles * 512];               // in lanes whose rows are not stored
     }
     float mn = mx;
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) mn = fmaxf(mn, w[j].x);
+    for (int j = 0; j < kBatch; ++j) {
+      if (s0 + j >= p.splits) {                            // no such split: no row seen
+        w[j] = float2{kNone, 0.0f};
+        x[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      }
+      mn = fmaxf(mn, w[j].x);
+    }
     const float keep = mn == mx ? 1.0f : __builtin_amdgcn_exp2f(mx - mn);
     l *= keep;
     acc *= keep;
     mx = mn;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      if (w[j].x == kNone && w[j].y == 0.0f) continue;     // saw no row
-      const float a = w[j].x == mx ? 1.0f : __builtin_amdgcn_exp2f(w[j].x - mx);
+      const float a = w[j].x == mx ? 1.0f : __builtin_amdgcn_exp2f(w[j].x - mx);   // -inf: saw no row
       l += a * w[j].y;
       acc += a * x[j];
     }
   }
-  const float mo = __shfl_xor(mx, 32), mn = fmaxf(mx, mo);
-  const float a = mx == mn ? 1.0f : __builtin_amdgcn_exp2f(mx - mn), b = mo == mn ? 1.0f : __builtin_amdgcn_exp2f(mo - mn);
-  l = a * l + b * __shfl_xor(l, 32);
-  typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-  f16x4 y;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float sum = a * acc[e] + b * __shfl_xor(acc[e], 32);
-    y[e] = (_Float16)(l == 0.0f ? 0.0f : sum / l);
+  for (int i = 0; i < 4; ++i) rows_out[c * kOutRow + 32 * g + 8 * i + e] = (_Float16)(l == 0.0f ? 0.0f : acc[i] / l);
+  __syncthreads();
+  if (threadIdx.x < 256) {
+    const int q = threadIdx.x >> 4, d = 8 * (threadIdx.x & 15), r = r0 + q;
+    if (r < rows) {
+      const int t = row_node(r, group);
+      *reinterpret_cast<f16x8*>(p.out + t * p.out_stride + (kh * group + (r - t * group)) * 128 + d) =
+          *reinterpret_cast<const f16x8*>(rows_out + q * kOutRow + d);
+    }
   }
-  const int kh = i / rows, r = i % rows;
-  if (half == 0) *reinterpret_cast<f16x4*>(p.out + (r / group) * p.out_stride + (kh * group + r % group) * 128 + d) = y;
 }
 
 template <int kQ, int kQW, int kKW>
@@ -480,8 +489,8 @@ hipError_t launch_tree_attention(const TreeAttnParams& p, const TreeAttnPlan& pl
     default: e = launch<2, 4, 2>(p, plan.blocks, stream); break;
   }
   if (e != hipSuccess || plan.splits == 1) return e;
-  const int rows = p.nodes * p.heads;
-  hipLaunchKernelGGL(tree_attention_merge_kernel, dim3((rows + 3) / 4), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL(tree_attention_merge_kernel, dim3(plan.blocks * (plan.block_rows / 16), p.kv_heads), dim3(512), 0,
+                     stream, p, plan.block_rows);
   return hipGetLastError();
 }
 
