@@ -34,7 +34,6 @@ namespace {
 
 constexpr int kKeys = 32;
 constexpr float kLazy = 8.0f;            // log2 of the largest softmax weight before a rescale
-constexpr int kOutRow = 136;             // halves of an output row in LDS: 128, and 8 to spread the banks
 __device__ constexpr float kNone = -__builtin_inff();
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -413,61 +412,63 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
   }
 }
 
-// Folds the splits of 16 query rows of one cache head: a wave per fragment e, all of its splits'
-// loads of a batch in flight.
-__global__ __launch_bounds__(512) void tree_attention_merge_kernel(TreeAttnParams p, int block_rows) {
-  __shared__ __align__(16) _Float16 rows_out[16 * kOutRow];
-  constexpr int kBatch = 16;
-  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  const int e = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int tiles = block_rows / 16, tile = blockIdx.x % tiles, block = blockIdx.x / tiles, kh = blockIdx.y;
-  const int group = p.heads / p.kv_heads, rows = p.nodes * group;
-  const int r0 = block * block_rows + 16 * tile;
-  if (r0 >= rows) return;
-  const long long slot = (long long)(block * p.kv_heads + kh) * p.splits;
-  const f32x4* po = p.part_o + ((slot * tiles + tile) * 8 + e) * 64 + lane;   // splits tiles * 8 * 64 apart
-  const float2* ml = p.part_ml + slot * block_rows + 16 * tile + c;
+// Folds the splits of 16 query rows of one cache head: a wave for the fragments 2 x and 2 x + 1
+// of a block's row tile, so that a few rows are spread over many CUs; kBatch splits' loads are
+// in flight together.  (Rows that are not there: whatever the workspace holds, in lanes that
+// store nothing.)
+template <int kBatch>
+__global__ __launch_bounds__(64) void tree_attention_merge_kernel(TreeAttnParams p) {
+  const int lane = threadIdx.x, c = lane & 15, g = lane >> 4;
+  const int pair = blockIdx.x & 3, tile = blockIdx.x >> 2, tiles = gridDim.x >> 2, kh = blockIdx.y;
+  const int group = p.heads / p.kv_heads;
+  const int r = (blockIdx.z * tiles + tile) * 16 + c;
+  const long long slot = (long long)(blockIdx.z * p.kv_heads + kh) * p.splits;
+  const f32x4* po = p.part_o + ((slot * tiles + tile) * 8 + 2 * pair) * 64 + lane;   // a split: tiles * 512
+  const float2* ml = p.part_ml + (slot * tiles + tile) * 16 + c;                     // a split: tiles * 16
   float mx = kNone, l = 0.0f;
-  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  f32x4 a0 = {0.0f, 0.0f, 0.0f, 0.0f}, a1 = a0;
   for (int s0 = 0; s0 < p.splits; s0 += kBatch) {
     float2 w[kBatch];
-    f32x4 x[kBatch];
+    f32x4 x[kBatch], y[kBatch];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       const int s = min(s0 + j, p.splits - 1);
-      w[j] = ml[(long long)s * block_rows];                // rows that are not there: whatever the workspace holds,
-      x[j] = po[(long long)s * tiles * 512];               // in lanes whose rows are not stored
+      w[j] = ml[s * tiles * 16];
+      x[j] = po[s * tiles * 512];
+      y[j] = po[s * tiles * 512 + 64];
     }
     float mn = mx;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       if (s0 + j >= p.splits) {                            // no such split: no row seen
         w[j] = float2{kNone, 0.0f};
-        x[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        x[j] = y[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       }
       mn = fmaxf(mn, w[j].x);
     }
     const float keep = mn == mx ? 1.0f : __builtin_amdgcn_exp2f(mx - mn);
     l *= keep;
-    acc *= keep;
+    a0 *= keep;
+    a1 *= keep;
     mx = mn;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       const float a = w[j].x == mx ? 1.0f : __builtin_amdgcn_exp2f(w[j].x - mx);   // -inf: saw no row
       l += a * w[j].y;
-      acc += a * x[j];
+      a0 += a * x[j];
+      a1 += a * y[j];
     }
   }
+  if (r >= p.nodes * group) return;
+  const int t = row_node(r, group);
+  const float inv = 1.0f / l;
+  _Float16* out = reinterpret_cast<_Float16*>(p.out) + t * p.out_stride + (kh * group + (r - t * group)) * 128 + 32 * g + 2 * pair;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) rows_out[c * kOutRow + 32 * g + 8 * i + e] = (_Float16)(l == 0.0f ? 0.0f : acc[i] / l);
-  __syncthreads();
-  if (threadIdx.x < 256) {
-    const int q = threadIdx.x >> 4, d = 8 * (threadIdx.x & 15), r = r0 + q;
-    if (r < rows) {
-      const int t = row_node(r, group);
-      *reinterpret_cast<f16x8*>(p.out + t * p.out_stride + (kh * group + (r - t * group)) * 128 + d) =
-          *reinterpret_cast<const f16x8*>(rows_out + q * kOutRow + d);
-    }
+  for (int i = 0; i < 4; ++i) {
+    f16x2 v;
+    v[0] = (_Float16)(l == 0.0f ? 0.0f : a0[i] * inv);
+    v[1] = (_Float16)(l == 0.0f ? 0.0f : a1[i] * inv);
+    *reinterpret_cast<f16x2*>(out + 8 * i) = v;
   }
 }
 
@@ -489,8 +490,13 @@ hipError_t launch_tree_attention(const TreeAttnParams& p, const TreeAttnPlan& pl
     default: e = launch<2, 4, 2>(p, plan.blocks, stream); break;
   }
   if (e != hipSuccess || plan.splits == 1) return e;
-  hipLaunchKernelGGL(tree_attention_merge_kernel, dim3(plan.blocks * (plan.block_rows / 16), p.kv_heads), dim3(512), 0,
-                     stream, p, plan.block_rows);
+  const dim3 grid(4 * (plan.block_rows / 16), p.kv_heads, plan.blocks);
+  if (plan.splits <= 4)
+    hipLaunchKernelGGL(tree_attention_merge_kernel<4>, grid, dim3(64), 0, stream, p);
+  else if (plan.splits <= 8)
+    hipLaunchKernelGGL(tree_attention_merge_kernel<8>, grid, dim3(64), 0, stream, p);
+  else
+    hipLaunchKernelGGL(tree_attention_merge_kernel<16>, grid, dim3(64), 0, stream, p);
   return hipGetLastError();
 }
 
