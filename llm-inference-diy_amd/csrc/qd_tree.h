@@ -66,8 +66,10 @@ struct TreeAttnPlan {
 inline TreeAttnPlan tree_attn_plan(int nodes, int heads, int kv_heads, int prefix, int num_cus, int* max_splits) {
   TreeAttnPlan plan;
   const int rows = nodes * (heads / kv_heads);
-  plan.block_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-  plan.key_waves = rows <= 32 ? 8 : rows <= 64 ? 4 : 2;
+  // 128-row blocks unless 64-row blocks leave fewer rows empty
+  const bool wide = (rows + 127) / 128 * 2 == (rows + 63) / 64;
+  plan.block_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : wide ? 128 : 64;
+  plan.key_waves = rows <= 32 ? 8 : wide ? 2 : 4;
   plan.blocks = (rows + plan.block_rows - 1) / plan.block_rows;
   const int most = num_cus / (plan.blocks * kv_heads);
   *max_splits = most < 1 ? 1 : most;

@@ -37,7 +37,6 @@ constexpr float kLazy = 8.0f;            // log2 of the largest softmax weight b
 __device__ constexpr float kNone = -__builtin_inff();
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 // What a lane holds of a V tile: dims 8 c .. 8 c + 7 of rows 4 j + g.
 struct Rows {
@@ -53,16 +52,6 @@ __device__ __forceinline__ f16x8 v_column(const u32x4 (&v)[8], int e) {
   return __builtin_bit_cast(f16x8, r);
 }
 
-__device__ __forceinline__ bool any_nonfinite(const u32x4 (&v)[8]) {
-  u16x2 m = {0, 0};
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[i][j] & 0x7fff7fffu));
-  return m[0] >= 0x7c00 || m[1] >= 0x7c00;
-}
-
 // A descriptor of wave-uniform values, held in scalar registers.
 __device__ __forceinline__ i32x4 wave_rsrc(const void* base, unsigned bytes) {
   i32x4 r = buffer_rsrc(base, bytes);
@@ -70,6 +59,23 @@ __device__ __forceinline__ i32x4 wave_rsrc(const void* base, unsigned bytes) {
   r[1] = __builtin_amdgcn_readfirstlane(r[1]);
   r[2] = __builtin_amdgcn_readfirstlane(r[2]);
   return r;
+}
+
+// Whether any half of x is an infinity or a NaN; x with those halves cleared.
+__device__ __forceinline__ bool has_nonfinite(u32x4 x) {
+  bool bad = false;
+#pragma unroll
+  for (int d = 0; d < 4; ++d) bad |= (x[d] & 0x7c00u) == 0x7c00u || (x[d] & 0x7c000000u) == 0x7c000000u;
+  return bad;
+}
+__device__ __forceinline__ u32x4 finite_halves(u32x4 x) {
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    unsigned keep = (x[d] & 0x7c00u) == 0x7c00u ? 0xffff0000u : 0xffffffffu;
+    if ((x[d] & 0x7c000000u) == 0x7c000000u) keep &= 0x0000ffffu;
+    x[d] &= keep;
+  }
+  return x;
 }
 
 // Node of query row r (row = node * group + head of the group): exact for rows below 2^22 (the
@@ -86,7 +92,7 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
   constexpr int kRows = 16 * kQ * kQW;                   // query rows of the block
   constexpr int kThreads = kQW * kKW * 64;
   // K (and shared V) tiles during the scan, the waves' accumulators afterwards.
-  constexpr size_t kTiles = kQW == 1 ? (size_t)kKW * kKeys * 256 : (size_t)2 * kKW * kKeys * 512;
+  constexpr size_t kTiles = (size_t)(kQW == 1 ? 1 : 4) * kKW * kKeys * 256;
   constexpr size_t kFold = (size_t)kKW * kRows * (128 * 4 + 8) + kQW * kKW * 4;
   __shared__ __align__(16) char smem[kTiles > kFold ? kTiles : kFold];
   const int lane = threadIdx.x & 63;
@@ -194,19 +200,36 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
   // exactly the loads that they need.
   const int cache_tiles = (p.prefix + kKeys - 1) / kKeys;
   const int tiles = cache_tiles + (p.nodes + kKeys - 1) / kKeys;
+  const int step = p.splits * kKW;                         // tiles from one of a wave's to its next
+  int tile = split * kKW + kw;
   struct Source {
     i32x4 k, v;
     unsigned off, row4;
   };
+  // Descriptors of tile t; called for the wave's tiles in turn.  The cache's whole tiles lie a
+  // constant apart.
+  const int full = p.prefix / kKeys;
+  const uint16_t* k_next = p.k + kh * p.head_stride + (long long)tile * kKeys * p.row_stride;
+  const uint16_t* v_next = p.v + kh * p.head_stride + (long long)tile * kKeys * p.row_stride;
+  const long long hop = (long long)step * kKeys * p.row_stride;
   auto source = [&](int t) {
-    const bool node = t >= cache_tiles;
-    const int row = (node ? t - cache_tiles : t) * kKeys, left = (node ? p.nodes : p.prefix) - row;
-    const long long stride = node ? p.trow_stride : p.row_stride, head = kh * (node ? p.thead_stride : p.head_stride);
-    const unsigned row_bytes = (unsigned)(stride * 2);
-    const unsigned bytes = t >= tiles ? 0u : (unsigned)(min(left, kKeys) - 1) * row_bytes + 256u;
+    const uint16_t *kb = k_next, *vb = v_next;
+    unsigned row_bytes = (unsigned)(p.row_stride * 2), bytes = 0xffffffffu;
+    if (t >= full) {
+      const bool node = t >= cache_tiles;
+      const int row = (node ? t - cache_tiles : t) * kKeys, left = (node ? p.nodes : p.prefix) - row;
+      if (node) {
+        kb = p.kt + kh * p.thead_stride + row * p.trow_stride;
+        vb = p.vt + kh * p.thead_stride + row * p.trow_stride;
+        row_bytes = (unsigned)(p.trow_stride * 2);
+      }
+      bytes = t >= tiles ? 0u : (unsigned)(min(left, kKeys) - 1) * row_bytes + 256u;
+    }
+    k_next += hop;
+    v_next += hop;
     Source x;
-    x.k = wave_rsrc((node ? p.kt : p.k) + head + row * stride, bytes);
-    x.v = wave_rsrc((node ? p.vt : p.v) + head + row * stride, bytes);
+    x.k = wave_rsrc(kb, bytes);
+    x.v = wave_rsrc(vb, bytes);
     x.off = (unsigned)g * row_bytes + 16u * c;
     x.row4 = 4u * row_bytes;
     return x;
@@ -233,18 +256,16 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
       for (int s = 0; s < 4; ++s)
         k[4 * a + s] = *reinterpret_cast<const u32x4*>(lk + (16 * a + krow) * 256 + 16 * ((4 * s + g) ^ krow));
   };
-  bool nonfinite = false;                                  // a node tile held infinities or NaN
-  // Scores, weights and products of one tile; `values` delivers the V rows when they are wanted.
-  auto tile_step = [&](int t, const char* lk, auto&& values) {
+  // Weights of tile t from its K rows in LDS.
+  auto weigh = [&](int t, const char* lk, f16x8 (&pb)[kQ]) {
     f32x4 st[kQ][2];
-    f16x8 pb[kQ];
     {
       u32x4 k[8];
       get_k(lk, k);
       scores(k, st);
     }
-    const bool node = t >= cache_tiles;
-    if (node || (t + 1) * kKeys > p.prefix) {              // node rows, or the cache's last rows
+    if ((t + 1) * kKeys > p.prefix) {                      // node rows, or the cache's last rows
+      const bool node = t >= cache_tiles;
       const int n = node ? p.nodes - (t - cache_tiles) * kKeys : p.prefix - t * kKeys;
       const unsigned rows_here = n >= kKeys ? ~0u : (1u << n) - 1u;
 #pragma unroll
@@ -255,27 +276,21 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
       }
     }
     weights(st, pb);
-    Rows v;
-    values(v);
-    // A weight of 0 keeps a finite V row out of a product, but not an infinity or a NaN: in a
-    // node tile such elements count as 0, and the fold adds them where they are seen.
-    if (node && __any(any_nonfinite(v.x))) {
-      nonfinite = true;
+  };
+  // A weight of 0 keeps a finite V row out of a product, but not an infinity or a NaN: in a node
+  // tile such elements count as 0, and the fold adds them where they are seen.
+  bool nonfinite = false;
+  auto make_finite = [&](auto& v) {
+    constexpr int n = sizeof(v) / sizeof(u32x4);
+    bool bad = false;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < n; ++i) bad |= has_nonfinite(v[i]);
+    if (!__any(bad)) return;
+    nonfinite = true;
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {
-          const unsigned x = v.x[i][d];
-          unsigned keep = (x & 0x7c00u) == 0x7c00u ? 0xffff0000u : 0xffffffffu;
-          if ((x & 0x7c000000u) == 0x7c000000u) keep &= 0x0000ffffu;
-          v.x[i][d] = x & keep;
-        }
-    }
-    products(v, pb);
+    for (int i = 0; i < n; ++i) v[i] = finite_halves(v[i]);
   };
 
-  const int step = p.splits * kKW;
-  int tile = split * kKW + kw;
   if constexpr (kQW == 1) {
     // A wave's own tiles: K through its own LDS rows (in order within the wave, no barrier),
     // V straight to registers.
@@ -295,7 +310,10 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
       const Source next = source(tile + step);
 #pragma unroll
       for (int j = 0; j < 8; ++j) kr[j] = load_k(next, j);
-      tile_step(tile, lk, [&](Rows& x) { x = v; });
+      f16x8 pb[kQ];
+      weigh(tile, lk, pb);
+      if (tile >= cache_tiles) make_finite(v.x);
+      products(v, pb);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v.x[j] = load_v(next, j);
     }
@@ -305,6 +323,7 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
     // written again only after the barrier behind its readers).  All key groups run the
     // same number of rounds.
     constexpr int kPart = 8 / kQW;
+    constexpr int kTile = kKeys * 256;                     // bytes of a K or V tile
     const int qw = wave % kQW;
     const int rounds = (tiles - split * kKW + step - 1) / step;
     const bool active = r0 + wq0 < rows;
@@ -316,10 +335,10 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
 #pragma unroll
       for (int j = 0; j < kPart; ++j) v[j] = load_v(x, kPart * qw + j);
     };
-    auto round = [&](int it, int buf, u32x4 (&kx)[kPart], u32x4 (&vx)[kPart]) {
-      char* lk = smem + (buf * kKW + kw) * kKeys * 512;
-      char* lv = lk + kKeys * 256;
-      const int t = tile + it * step;
+    auto round = [&](int t, int buf, u32x4 (&kx)[kPart], u32x4 (&vx)[kPart]) {
+      char* lk = smem + (buf * kKW + kw) * 2 * kTile;
+      char* lv = lk + kTile;
+      if (t >= cache_tiles) make_finite(vx);
 #pragma unroll
       for (int j = 0; j < kPart; ++j) {
         put_k(lk, kPart * qw + j, kx[j]);
@@ -327,17 +346,21 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
       }
       fetch(t + 2 * step, kx, vx);
       __syncthreads();
-      if (active && t < tiles)
-        tile_step(t, lk, [&](Rows& v) {
+      if (active && t < tiles) {
+        f16x8 pb[kQ];
+        weigh(t, lk, pb);
+        Rows v;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v.x[j] = *reinterpret_cast<const u32x4*>(lv + (4 * j + g) * 256 + 16 * c);
-        });
+        for (int j = 0; j < 8; ++j) v.x[j] = *reinterpret_cast<const u32x4*>(lv + (4 * j + g) * 256 + 16 * c);
+        products(v, pb);
+      }
     };
     fetch(tile, kr[0], vr[0]);
     fetch(tile + step, kr[1], vr[1]);
     for (int it = 0; it < rounds; it += 2) {               // an odd count's last round finds no tile
-      round(it, 0, kr[0], vr[0]);
-      round(it + 1, 1, kr[1], vr[1]);
+      round(tile, 0, kr[0], vr[0]);
+      round(tile + step, 1, kr[1], vr[1]);
+      tile += 2 * step;
     }
   }
   // Fold the key waves.  Every wave leaves its accumulators in LDS as they lie in its registers
@@ -360,42 +383,55 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) any_bad |= bad[w] != 0;
   const int slot = (blockIdx.z * p.kv_heads + kh) * p.splits + split;
-  for (int f = wave; f < kFrags; f += kWaves) {
-    const int e = f & 7, q = 16 * (f >> 3) + c;            // the lane's row in the block
-    float mx = kNone, l = 0.0f;
-    float2 ml[kKW];
+  // A wave's fragments belong to one tile of 16 rows: the key waves' weights are formed once.
+  constexpr int kOwn = kFrags / kWaves;
+  static_assert(8 % kOwn == 0, "a wave's fragments lie in one row tile");
+  const int f0 = wave * kOwn, q = 16 * (f0 >> 3) + c;      // the lane's row in the block
+  float mx = kNone, l = 0.0f, a[kKW];
 #pragma unroll
-    for (int w = 0; w < kKW; ++w) {
-      ml[w] = state[w * kRows + q];
-      mx = fmaxf(mx, ml[w].x);
-    }
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int w = 0; w < kKW; ++w) mx = fmaxf(mx, state[w * kRows + q].x);
 #pragma unroll
-    for (int w = 0; w < kKW; ++w) {
-      const float a = ml[w].x == mx ? 1.0f : __builtin_amdgcn_exp2f(ml[w].x - mx);   // -inf: saw no row
-      l += a * ml[w].y;
-      acc += a * frag[(w * kFrags + f) * 64 + lane];
-    }
-    const int r = min(r0 + q, rows - 1);
-    if (any_bad) {                                         // infinities and NaN of this workgroup's node tiles
-      const uint64_t* mask = p.mask + (long long)row_node(r, group) * words;
-      for (int j = 0; j < p.nodes; ++j) {
-        if ((cache_tiles + j / kKeys) % step / kKW != split || !((mask[j >> 6] >> (j & 63)) & 1u)) continue;
-        const uint16_t* v = p.vt + kh * p.thead_stride + j * p.trow_stride + 32 * g + e;
+  for (int w = 0; w < kKW; ++w) {
+    const float2 ml = state[w * kRows + q];
+    a[w] = ml.x == mx ? 1.0f : __builtin_amdgcn_exp2f(ml.x - mx);   // -inf: saw no row
+    l += a[w] * ml.y;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const bool live = r0 + q < rows;
+  if (any_bad) {
+    // Add the infinities and NaN of this workgroup's node tiles that the row sees, to the
+    // accumulators of a key wave whose weight is 1.
+    int one = 0;
+#pragma unroll
+    for (int w = 0; w < kKW; ++w) one = a[w] == 1.0f ? w : one;
+    const uint64_t* mask = p.mask + (long long)row_node(min(r0 + q, rows - 1), group) * words;
+#pragma unroll 1
+    for (int j = 0; j < p.nodes; ++j) {
+      if ((cache_tiles + j / kKeys) % step / kKW != split || !((mask[j >> 6] >> (j & 63)) & 1u)) continue;
+#pragma unroll 1
+      for (int f = f0; f < f0 + kOwn; ++f) {
+        const uint16_t* v = p.vt + kh * p.thead_stride + j * p.trow_stride + 32 * g + (f & 7);
+        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float x = (float)*reinterpret_cast<const _Float16*>(v + 8 * i);
-          if (!(fabsf(x) < __builtin_inff())) acc[i] += x;
+          const float y = (float)*reinterpret_cast<const _Float16*>(v + 8 * i);
+          x[i] = fabsf(y) < __builtin_inff() ? 0.0f : y;
         }
+        frag[(one * kFrags + f) * 64 + lane] += x;
       }
     }
+  }
+  if (p.splits > 1 && live && (f0 & 7) == 0 && g == 0) p.part_ml[(long long)slot * kRows + q] = float2{mx, l};
+#pragma unroll
+  for (int n = 0; n < kOwn; ++n) {
+    const int f = f0 + n;
+    f32x4 acc = a[0] * frag[f * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < kKW; ++w) acc += a[w] * frag[(w * kFrags + f) * 64 + lane];
     if (p.splits > 1) {
-      if (r0 + q < rows) {
-        p.part_o[((long long)slot * kFrags + f) * 64 + lane] = acc;
-        if (e == 0 && g == 0) p.part_ml[(long long)slot * kRows + q] = float2{mx, l};
-      }
+      if (live) p.part_o[((long long)slot * kFrags + f) * 64 + lane] = acc;
     } else {
-      frag[f * 64 + lane] = l == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc / l;   // read by this wave alone
+      frag[f * 64 + lane] = l == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc * inv;   // read by this wave alone
     }
   }
   if (p.splits > 1) return;
