@@ -180,8 +180,8 @@ int qd_tree_attention(qd_ctx* ctx, const uint16_t* q, long long q_stride, const 
   float2* part_ml = reinterpret_cast<float2*>(part_o + (size_t)plan.blocks * kvh * max_splits * plan.block_rows * 128);
   const qd::TreeAttnParams p{q, k_layer, v_layer, k_tree, v_tree, mask, out, q_stride, out_stride,
                              ctx->cfg.kv_row_stride, ctx->cfg.kv_head_stride, tree_row_stride, tree_head_stride,
-                             prefix, nodes, num_heads, kvh, (float)(1.4426950408889634 / std::sqrt(128.0)),
-                             plan.splits, reinterpret_cast<decltype(qd::TreeAttnParams::part_o)>(part_o), part_ml};
+                             prefix, nodes, kvh, num_heads / kvh, (float)(1.4426950408889634 / std::sqrt(128.0)),
+                             plan.splits, plan.rounds, plan.block_rows, reinterpret_cast<decltype(qd::TreeAttnParams::part_o)>(part_o), part_ml};
   const hipError_t e = qd::launch_tree_attention(p, plan, stream);
   return e == hipSuccess ? QD_OK : hip_fail(e, "tree attention launch");
 }

@@ -46,9 +46,10 @@ struct TreeAttnParams {
   long long q_stride, out_stride;
   long long row_stride, head_stride;      // cache
   long long trow_stride, thead_stride;    // node rows
-  int prefix, nodes, heads, kv_heads;
+  int prefix, nodes, kv_heads;
+  int group;                // query heads per cache head
   float scale_log2;         // log2(e) / sqrt(128)
-  int splits;               // workgroups per block of query rows (TreeAttnPlan)
+  int splits, rounds, block_rows;   // TreeAttnPlan
   // Partials, when splits > 1, per (block, cache head, split): the block's accumulators as
   // fragments [block_rows / 16][8][64 lanes], and its rows' (log2 reference, denominator).
   float __attribute__((ext_vector_type(4)))* part_o;
@@ -59,7 +60,7 @@ struct TreeAttnParams {
 // its nodes x the heads that share it), `splits` workgroups of eight waves for each, of which
 // key_waves take different tiles of keys.
 struct TreeAttnPlan {
-  int block_rows, key_waves, blocks, splits;
+  int block_rows, key_waves, blocks, splits, rounds;   // rounds: tiles of a key wave, at most
 };
 
 // max_splits: what the workspace is sized for, at any prefix.
@@ -76,6 +77,7 @@ inline TreeAttnPlan tree_attn_plan(int nodes, int heads, int kv_heads, int prefi
   const int tiles = (prefix + 31) / 32 + (nodes + 31) / 32;
   const int by_tiles = (tiles + plan.key_waves - 1) / plan.key_waves;
   plan.splits = *max_splits < by_tiles ? *max_splits : by_tiles;
+  plan.rounds = (by_tiles + plan.splits - 1) / plan.splits;
   return plan;
 }
 hipError_t launch_tree_attention(const TreeAttnParams& p, const TreeAttnPlan& plan, hipStream_t stream);

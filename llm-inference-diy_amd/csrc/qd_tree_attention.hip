@@ -78,6 +78,13 @@ __device__ __forceinline__ u32x4 finite_halves(u32x4 x) {
   return x;
 }
 
+// Touches the argument block's three cache lines at once: on its own the compiler loads each
+// argument where it is first used, and waits for a line three times in a row.
+__device__ __forceinline__ void load_arguments(const TreeAttnParams& p) {
+  static_assert(sizeof(TreeAttnParams) > 128 && sizeof(TreeAttnParams) <= 192, "three 64-byte lines");
+  asm volatile("" ::"s"(p.q), "s"(p.q_stride), "s"(p.part_o));
+}
+
 // Node of query row r (row = node * group + head of the group): exact for rows below 2^22 (the
 // reciprocal's estimate is off by at most one).
 __device__ __forceinline__ int row_node(int r, int group) {
@@ -99,9 +106,10 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int kw = wave / kQW, wq0 = 16 * kQ * (wave % kQW);   // key group, first row in the block
   const int c = lane & 15, g = lane >> 4;
+  load_arguments(p);
   const int split = blockIdx.x, kh = blockIdx.y;
   const int r0 = blockIdx.z * kRows;                     // the block's first query row
-  const int group = p.heads / p.kv_heads;
+  const int group = p.group;
   const int rows = p.nodes * group;
   const int words = (p.nodes + 63) / 64;
 
@@ -325,7 +333,6 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
     constexpr int kPart = 8 / kQW;
     constexpr int kTile = kKeys * 256;                     // bytes of a K or V tile
     const int qw = wave % kQW;
-    const int rounds = (tiles - split * kKW + step - 1) / step;
     const bool active = r0 + wq0 < rows;
     u32x4 kr[2][kPart], vr[2][kPart];
     auto fetch = [&](int t, u32x4 (&k)[kPart], u32x4 (&v)[kPart]) {
@@ -357,8 +364,9 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
     };
     fetch(tile, kr[0], vr[0]);
     fetch(tile + step, kr[1], vr[1]);
-    for (int it = 0; it < rounds; it += 2) {               // an odd count's last round finds no tile
+    for (int it = 0; it < p.rounds; it += 2) {
       round(tile, 0, kr[0], vr[0]);
+      if (it + 1 == p.rounds) break;
       round(tile + step, 1, kr[1], vr[1]);
       tile += 2 * step;
     }
@@ -455,8 +463,9 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
 template <int kBatch>
 __global__ __launch_bounds__(64) void tree_attention_merge_kernel(TreeAttnParams p) {
   const int lane = threadIdx.x, c = lane & 15, g = lane >> 4;
-  const int pair = blockIdx.x & 3, tile = blockIdx.x >> 2, tiles = gridDim.x >> 2, kh = blockIdx.y;
-  const int group = p.heads / p.kv_heads;
+  load_arguments(p);
+  const int pair = blockIdx.x & 3, tile = blockIdx.x >> 2, tiles = p.block_rows >> 4, kh = blockIdx.y;
+  const int group = p.group;
   const int r = (blockIdx.z * tiles + tile) * 16 + c;
   const long long slot = (long long)(blockIdx.z * p.kv_heads + kh) * p.splits;
   const f32x4* po = p.part_o + ((slot * tiles + tile) * 8 + 2 * pair) * 64 + lane;   // a split: tiles * 512
