@@ -188,7 +188,8 @@ int qd_tree_attention(qd_ctx* ctx, const uint16_t* q, long long q_stride, const 
 
 size_t qd_tree_verify_workspace_bytes(int nodes, int vocab, int max_children) {
   if (!verify_args_ok(nodes, vocab, max_children)) return 0;
-  const size_t rows = (size_t)nodes * qd::verify_chunks(vocab);
+  const int chunk = qd::verify_chunk(nodes, vocab);
+  const size_t rows = (size_t)nodes * ((vocab + chunk - 1) / chunk);
   return round16(2 * rows * sizeof(double)) + round16((size_t)max_children * rows * sizeof(double)) +
          round16(2 * rows * sizeof(float)) + round16(rows * sizeof(int));
 }
@@ -249,7 +250,8 @@ int qd_tree_verify(const uint16_t* target_logits, long long ldt, const uint16_t*
   p.scale_log2 = greedy ? 0.0 : 1.4426950408889634 / (double)temperature;
   p.nodes = nodes;
   p.vocab = vocab;
-  p.chunks = qd::verify_chunks(vocab);
+  p.chunk = qd::verify_chunk(nodes, vocab);
+  p.chunks = (vocab + p.chunk - 1) / p.chunk;
   p.max_children = nodes > 1 ? max_children : 0;
   p.greedy = greedy;
   const size_t rows = (size_t)nodes * p.chunks;

@@ -82,9 +82,9 @@ inline TreeAttnPlan tree_attn_plan(int nodes, int heads, int kv_heads, int prefi
 }
 hipError_t launch_tree_attention(const TreeAttnParams& p, const TreeAttnPlan& plan, hipStream_t stream);
 
-// Logits of a row per workgroup of the verification's passes over them.
-constexpr int kVerifyChunk = 8192;
-inline int verify_chunks(int vocab) { return (vocab + kVerifyChunk - 1) / kVerifyChunk; }
+// Logits of a row per workgroup of the verification's passes over them: 8192, or 2048 where
+// that leaves the chip's CUs half empty.
+inline int verify_chunk(int nodes, int vocab) { return (long long)nodes * ((vocab + 8191) / 8192) >= 512 ? 8192 : 2048; }
 
 struct TreeVerifyParams {
   const uint16_t* target;   // [nodes][vocab]
@@ -105,7 +105,7 @@ struct TreeVerifyParams {
   int* args;                // [nodes][chunks]
   long long ldt, ldd;
   double scale_log2;        // log2(e) / temperature
-  int nodes, vocab, chunks, max_children;
+  int nodes, vocab, chunk, chunks, max_children;
   int greedy;
 };
 hipError_t launch_tree_verify(const TreeVerifyParams& p, hipStream_t stream);

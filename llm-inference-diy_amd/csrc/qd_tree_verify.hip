@@ -13,12 +13,12 @@
 //   A_{j+1} = A_j + S_j,   S_{j+1} = sum_v max(p(v) - A_{j+1} q(v), 0),
 // since max(p - A_j q, 0)/S_j - q = (p - (A_j + S_j) q)/S_j wherever it is positive.
 //
-// Passes: (1) every (row, chunk of kVerifyChunk logits) gives its largest logit
-// and its sum of weights relative to it, or its argmax; (2) with drawn drafts,
-// per round j <= max_children, the chunks' sums of S_j, for every node with at
-// least j children; (3) one workgroup reduces the rows' partials, decides every
-// node's children (a node's decisions do not depend on how it was reached), walks
-// from node 0, and takes the last token from one chunk.
+// Passes: (1) every (row, chunk of logits) gives its largest logit and its sum of weights
+// relative to it, or its argmax; (2) with drawn drafts, per round j <= max_children, the
+// chunks' sums of S_j, for every node whose first j children are all rejected; (3) one
+// workgroup reduces the rows' partials, decides every node's children (a node's decisions do
+// not depend on how it was reached), walks from node 0, and takes the last token from one
+// chunk.
 #include "qd_device.h"
 #include "qd_internal.h"
 #include "qd_tree.h"
@@ -30,32 +30,45 @@ namespace {
 typedef _Float16 f16x8u __attribute__((ext_vector_type(8), aligned(2)));   // rows need not be 16-byte aligned
 
 constexpr int kNodes = QD_TREE_MAX_NODES;
+constexpr int kThreads = 256;                          // of the passes over chunks: runs of 8 logits per thread
 
-// 2^x for x <= 0, relative error below 1e-12: 2^n times the Taylor series of
-// exp(f ln 2) to degree 10 on |f| <= 1/2 (remainder (ln2/2)^11 / 11! = 2e-13).
-// Below 2^-1000: 0.
-__device__ __forceinline__ double exp2_neg(double x) {
-  const double n = __builtin_rint(x);
-  const double f = (x - n) * 0.6931471805599453;
-  double r = 1.0 / 3628800.0;
-  r = __builtin_fma(r, f, 1.0 / 362880.0);
-  r = __builtin_fma(r, f, 1.0 / 40320.0);
-  r = __builtin_fma(r, f, 1.0 / 5040.0);
-  r = __builtin_fma(r, f, 1.0 / 720.0);
-  r = __builtin_fma(r, f, 1.0 / 120.0);
-  r = __builtin_fma(r, f, 1.0 / 24.0);
-  r = __builtin_fma(r, f, 1.0 / 6.0);
-  r = __builtin_fma(r, f, 0.5);
+// Weight of a logit in a row (or chunk): `m` its largest logit, `scale` log2(e) / temperature.
+struct Scale {
+  float m;
+  double md, scale;
+};
+__device__ __forceinline__ Scale make_scale(float m, double scale) { return Scale{m, (double)m, scale}; }
+
+// 2^x, x = (l - m) * scale <= 0, to a relative 1e-12: 2^n times the series of 2^f to degree 10 on
+// |f| <= 1/2 (remainder (ln2/2)^11 / 11! = 2e-13; the difference of two halves is exact).
+// Rounding to n by adding 1.5 * 2^52 leaves n in the low word, and adding n to the exponent
+// field scales: conversions, v_rndne_f64 and v_ldexp_f64 issue at a quarter of the rate of
+// v_fma_f64.  Below 2^-1000: 0, as for NaN (fmax drops it).  m is finite.
+__device__ __forceinline__ double weight_finite(float l, const Scale& s) {
+  const double x = fmax(((double)l - s.md) * s.scale, -1020.0);
+  const double t = x + 0x1.8p52;
+  const double f = x - (t - 0x1.8p52);
+  double r = 7.054911620801121e-09;                    // ln2^k / k!, k = 10 .. 0
+  r = __builtin_fma(r, f, 1.0178086009239699e-07);
+  r = __builtin_fma(r, f, 1.3215486790144307e-06);
+  r = __builtin_fma(r, f, 1.5252733804059838e-05);
+  r = __builtin_fma(r, f, 0.00015403530393381608);
+  r = __builtin_fma(r, f, 0.0013333558146428441);
+  r = __builtin_fma(r, f, 0.009618129107628477);
+  r = __builtin_fma(r, f, 0.05550410866482158);
+  r = __builtin_fma(r, f, 0.2402265069591007);
+  r = __builtin_fma(r, f, 0.6931471805599453);
   r = __builtin_fma(r, f, 1.0);
-  r = __builtin_fma(r, f, 1.0);
-  return x > -1000.0 ? __builtin_ldexp(r, (int)fmax(n, -1100.0)) : 0.0;
+  const long long bits = __builtin_bit_cast(long long, r);
+  const int lo = (int)bits, hi = (int)(bits >> 32) + ((int)__builtin_bit_cast(long long, t) << 20);
+  const double w = __builtin_bit_cast(double, ((long long)hi << 32) | (unsigned)lo);
+  return x > -1000.0 ? w : 0.0;
 }
-
-// Weight of logit l in a row (or chunk) whose largest logit is m; NaN counts as
-// -inf.  The largest itself weighs 1, also where it is infinite.
-__device__ __forceinline__ double weight(float l, float m, double scale) {
+// The same for any m: the largest logits weigh 1 also where they are infinite.
+__device__ __forceinline__ double weight(float l, const Scale& s) {
+  if (fabsf(s.m) < __builtin_inff()) return weight_finite(l, s);
   if (l != l) l = -__builtin_inff();
-  return l == m ? 1.0 : exp2_neg(((double)l - (double)m) * scale);
+  return l == s.m ? 1.0 : 0.0;
 }
 
 __device__ __forceinline__ double wave_sum(double x) {
@@ -76,36 +89,52 @@ __device__ __forceinline__ void load8(const uint16_t* row, int v, int vocab, flo
       x[e] = v + e < vocab ? (float)reinterpret_cast<const _Float16*>(row)[v + e] : -__builtin_inff();
   }
 }
+// Their weights; 0 past the row's end.
+__device__ __forceinline__ void weights8(const float (&x)[8], int v, int vocab, const Scale& s, double (&w)[8]) {
+  if (fabsf(s.m) < __builtin_inff()) {                 // uniform over a chunk
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = weight_finite(x[e], s);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = v + e < vocab ? weight(x[e], s) : 0.0;
+  }
+}
 
-constexpr int kThreads = 256;
-constexpr int kRuns = kVerifyChunk / (8 * kThreads);   // runs of 8 logits per thread
-
-// (1) Sampled: blockIdx = (chunk, node, side).
+// (1) Sampled: blockIdx = (chunk, node, side), a chunk kRuns runs per thread.  The drafter's
+// rows of nodes without children have no use.
+template <int kRuns>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(TreeVerifyParams p) {
   __shared__ float sm[kThreads / 64];
   __shared__ double ss[kThreads / 64];
   const int t = blockIdx.y, side = blockIdx.z, c = blockIdx.x;
   const uint16_t* row = side ? p.draft + t * p.ldd : p.target + t * p.ldt;
-  const int v0 = c * kVerifyChunk + 8 * threadIdx.x;
+  const int v0 = c * p.chunk + 8 * threadIdx.x;
   float x[kRuns][8];
+#pragma unroll
+  for (int r = 0; r < kRuns; ++r) load8(row, v0 + 8 * kThreads * r, p.vocab, x[r]);
+  if (side) {
+    bool child = false;
+    for (int s = t + 1 + threadIdx.x; s < p.nodes; s += kThreads) child |= p.parents[s] == t;
+    if (!__syncthreads_or(child)) return;
+  }
   float m = -__builtin_inff();
 #pragma unroll
-  for (int r = 0; r < kRuns; ++r) {
-    load8(row, v0 + 8 * kThreads * r, p.vocab, x[r]);
+  for (int r = 0; r < kRuns; ++r)
 #pragma unroll
     for (int e = 0; e < 8; ++e) m = fmaxf(m, x[r][e]);            // fmaxf passes NaN over
-  }
   m = wave64_max(m);
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kThreads / 64; ++w) m = fmaxf(m, sm[w]);
+  const Scale sc = make_scale(m, p.scale_log2);
   double s = 0.0;
 #pragma unroll
-  for (int r = 0; r < kRuns; ++r)
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (v0 + 8 * kThreads * r + e < p.vocab) s += weight(x[r][e], m, p.scale_log2);
+  for (int r = 0; r < kRuns; ++r) {
+    double w[8];
+    weights8(x[r], v0 + 8 * kThreads * r, p.vocab, sc, w);
+    s += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+  }
   s = wave_sum(s);
   if ((threadIdx.x & 63) == 0) ss[threadIdx.x >> 6] = s;
   __syncthreads();
@@ -125,22 +154,24 @@ __device__ __forceinline__ void better(float& m, int& i, float m2, int i2) {
     i = i2;
   }
 }
+template <int kRuns>
 __global__ __launch_bounds__(kThreads) void verify_argmax_kernel(TreeVerifyParams p) {
   __shared__ float sm[kThreads / 64];
   __shared__ int si[kThreads / 64];
   const int t = blockIdx.y, c = blockIdx.x;
   const uint16_t* row = p.target + t * p.ldt;
-  const int v0 = c * kVerifyChunk + 8 * threadIdx.x;
+  const int v0 = c * p.chunk + 8 * threadIdx.x;
+  float x[kRuns][8];
+#pragma unroll
+  for (int r = 0; r < kRuns; ++r) load8(row, v0 + 8 * kThreads * r, p.vocab, x[r]);
   float m = -__builtin_inff();
   int at = 0x7fffffff;
 #pragma unroll
   for (int r = 0; r < kRuns; ++r) {
-    float x[8];
     const int v = v0 + 8 * kThreads * r;
-    load8(row, v, p.vocab, x);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (v + e < p.vocab && x[e] == x[e]) better(m, at, x[e], v + e);
+      if (v + e < p.vocab && x[r][e] == x[r][e]) better(m, at, x[r][e], v + e);
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) better(m, at, __shfl_xor(m, d), __shfl_xor(at, d));
@@ -159,11 +190,15 @@ __global__ __launch_bounds__(kThreads) void verify_argmax_kernel(TreeVerifyParam
 // A row's largest logit and its sum of weights relative to it, by one wave.
 __device__ __forceinline__ void row_stats(const TreeVerifyParams& p, int side, int t, int lane, float& m, double& z) {
   const long long at = ((long long)side * p.nodes + t) * p.chunks;
-  m = -__builtin_inff();
-  for (int c = lane; c < p.chunks; c += 64) m = fmaxf(m, p.maxes[at + c]);
+  const bool first = lane < p.chunks;                  // the lane's first chunk, loaded once
+  const float m0 = first ? p.maxes[at + lane] : -__builtin_inff();
+  const double s0 = first ? p.sums[at + lane] : 0.0;
+  m = m0;
+  for (int c = lane + 64; c < p.chunks; c += 64) m = fmaxf(m, p.maxes[at + c]);
   m = wave64_max(m);
-  z = 0.0;
-  for (int c = lane; c < p.chunks; c += 64) z += p.sums[at + c] * weight(p.maxes[at + c], m, p.scale_log2);
+  const Scale sc = make_scale(m, p.scale_log2);
+  z = first ? s0 * weight(m0, sc) : 0.0;
+  for (int c = lane + 64; c < p.chunks; c += 64) z += p.sums[at + c] * weight(p.maxes[at + c], sc);
   z = wave_sum(z);
 }
 
@@ -175,61 +210,80 @@ __device__ __forceinline__ double round_total(const TreeVerifyParams& p, int r, 
   return wave_sum(z);
 }
 
-// A and S of a node after `rejected` rejections (rounds whose sum is 0 change
-// nothing), and the last round that counted (0: p itself).
+// The remaining distribution of a node with drawn drafts, max(p - a q, 0) / s, and the last
+// round that changed it (0: p itself).  A round whose sum is 0 changes nothing, nor does any
+// later one.
 struct Residual {
   double a, s;
   int round;
 };
-__device__ __forceinline__ Residual residual(const TreeVerifyParams& p, int t, int rejected, int lane) {
-  Residual r{0.0, 1.0, 0};
-  for (int j = 1; j <= rejected; ++j) {
-    const double s = round_total(p, j, t, lane);
-    if (s > 0.0) {
-      r.a += r.s;
-      r.s = s;
-      r.round = j;
-    } else {
-      break;                 // p stays as it was, and so does every later round's sum: 0
-    }
-  }
-  return r;
+__device__ __forceinline__ void reject(const TreeVerifyParams& p, int t, int rejected, int lane, Residual& r) {
+  if (r.round != rejected - 1) return;
+  const double s = round_total(p, rejected, t, lane);
+  if (s > 0.0) r = Residual{r.a + r.s, s, rejected};
 }
 
-// (2) Round `round` of drawn drafts: blockIdx = (chunk, node).
+__device__ __forceinline__ float logit(const uint16_t* row, int v) {
+  return (float)reinterpret_cast<const _Float16*>(row)[v];
+}
+// Probability of token x in a row; 0 outside the vocabulary.
+__device__ __forceinline__ double probability(const uint16_t* row, int x, int vocab, const Scale& s, double z) {
+  return x >= 0 && x < vocab ? weight(logit(row, x), s) / z : 0.0;
+}
+
+// (2) Round `round` of drawn drafts: blockIdx = (chunk, node).  Each wave finds out for itself
+// whether the node's first `round` children are all rejected; the chunk's logits are under way
+// meanwhile.
+template <int kRuns>
 __global__ __launch_bounds__(kThreads) void verify_round_kernel(TreeVerifyParams p, int round) {
   __shared__ double ss[kThreads / 64];
-  __shared__ int kids[kThreads / 64];
   const int t = blockIdx.y, c = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int n = 0;
-  for (int s = t + 1 + threadIdx.x; s < p.nodes; s += kThreads) n += p.parents[s] == t;
+  const uint16_t* rp = p.target + t * p.ldt;
+  const uint16_t* rq = p.draft + t * p.ldd;
+  int child = -1, found = 0;                           // lane k: the node's child k (from 0), k < round
+  for (int s0 = t + 1; s0 < p.nodes && found < round; s0 += 64) {
+    const int s = s0 + lane;
+    unsigned long long hits = __ballot(s < p.nodes && p.parents[s] == t);
+    for (; hits && found < round; hits &= hits - 1, ++found)
+      if (lane == found) child = s0 + __builtin_ctzll(hits);
+  }
+  if (found < round) return;                           // the same in every wave
+  const int v0 = c * p.chunk + 8 * threadIdx.x;
+  float x[kRuns][8], y[kRuns][8];
 #pragma unroll
-  for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
-  if (lane == 0) kids[wave] = n;
-  __syncthreads();
-  n = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) n += kids[w];
-  if (n < round) return;                             // uniform over the workgroup
+  for (int i = 0; i < kRuns; ++i) {
+    load8(rp, v0 + 8 * kThreads * i, p.vocab, x[i]);
+    load8(rq, v0 + 8 * kThreads * i, p.vocab, y[i]);
+  }
   float mp, mq;
   double zp, zq;
   row_stats(p, 0, t, lane, mp, zp);
   row_stats(p, 1, t, lane, mq, zq);
-  const Residual r = residual(p, t, round - 1, lane);
-  const bool kept = r.round != round - 1;            // an earlier round's sum was 0
-  const double a = (r.a + r.s) / zq, ip = 1.0 / zp;
-  const uint16_t* rp = p.target + t * p.ldt;
-  const uint16_t* rq = p.draft + t * p.ldd;
+  const Scale sp = make_scale(mp, p.scale_log2), sq = make_scale(mq, p.scale_log2);
+  double pw = 0.0, uq = 0.0, qw = 0.0;
+  if (child >= 0) {
+    const int tok = p.tokens[child];
+    pw = probability(rp, tok, p.vocab, sp, zp);
+    qw = probability(rq, tok, p.vocab, sq, zq);
+    uq = (double)p.accept_u[child] * qw;
+  }
+  Residual r{0.0, 1.0, 0};
+  for (int k = 0; k < round; ++k) {
+    const bool ok = __shfl(uq, k) * r.s < fmax(__shfl(pw, k) - r.a * __shfl(qw, k), 0.0);
+    if (ok) return;                                    // a child stands: no later round is looked at
+    if (k + 1 < round) reject(p, t, k + 1, lane, r);
+  }
   double s = 0.0;
-  if (!kept) {
-    for (int i = 0; i < kRuns; ++i) {
-      const int v = c * kVerifyChunk + 8 * (threadIdx.x + kThreads * i);
-      float x[8], y[8];
-      load8(rp, v, p.vocab, x);
-      load8(rq, v, p.vocab, y);
+  if (r.round == round - 1) {                          // else an earlier round's sum was 0
+    const double a = (r.a + r.s) / zq, ip = 1.0 / zp;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (v + e < p.vocab) s += fmax(weight(x[e], mp, p.scale_log2) * ip - weight(y[e], mq, p.scale_log2) * a, 0.0);
+    for (int i = 0; i < kRuns; ++i) {
+      const int v = v0 + 8 * kThreads * i;
+      double wp[8], wq[8];
+      weights8(x[i], v, p.vocab, sp, wp);
+      weights8(y[i], v, p.vocab, sq, wq);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += fmax(wp[e] * ip - wq[e] * a, 0.0);
     }
   }
   s = wave_sum(s);
@@ -241,23 +295,19 @@ __global__ __launch_bounds__(kThreads) void verify_round_kernel(TreeVerifyParams
   }
 }
 
-__device__ __forceinline__ float logit(const uint16_t* row, int v) {
-  return (float)reinterpret_cast<const _Float16*>(row)[v];
-}
-
 // (3) One workgroup.
 constexpr int kWalkThreads = 1024;
 constexpr int kWalkWaves = kWalkThreads / 64;
-constexpr int kPer = kVerifyChunk / kWalkThreads;      // 8 logits of the last chunk per thread
-static_assert(kPer == 8, "the last token's chunk is one run of 8 logits per thread");
+constexpr int kMaxChunk = 8 * kWalkThreads;            // the last token's chunk: 8 logits per thread
 
 struct WalkShared {
   int parent[kNodes], token[kNodes], next[kNodes], path[kNodes], best[kNodes];
-  float mp[kNodes], mq[kNodes];
+  float mp[kNodes], mq[kNodes], u[kNodes];
   double zp[kNodes], zq[kNodes];
+  double pw[kNodes], qw[kNodes];                       // a node's token in its parent's distributions
   double wave[kWalkWaves];
-  unsigned gone[kVerifyChunk / 32];                    // rejected tokens of one chunk
-  int count, chunk, last;
+  unsigned gone[kMaxChunk / 32];                       // rejected tokens of one chunk
+  int count, chunk, first, tail;
   double before, total;
 };
 
@@ -277,10 +327,12 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
   __shared__ WalkShared sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const bool drawn = !p.greedy && p.draft != nullptr;
+  const float sample_u = p.greedy ? 0.0f : *p.sample_u;
   for (int t = tid; t < p.nodes; t += kWalkThreads) {
-    sh.parent[t] = t ? p.parents[t] : -1;
-    if (t && sh.parent[t] >= t) sh.parent[t] = -1;      // never reached
+    const int parent = t ? p.parents[t] : -1;
+    sh.parent[t] = parent < t ? parent : -1;           // otherwise never reached
     sh.token[t] = t ? p.tokens[t] : -1;
+    sh.u[t] = t && !p.greedy ? p.accept_u[t] : 0.0f;
     sh.next[t] = -1;
   }
   for (int t = wave; t < p.nodes; t += kWalkWaves) {
@@ -300,7 +352,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
         sh.mp[t] = m;
         sh.zp[t] = z;
       }
-      if (drawn) {
+      if (drawn) {                                     // of a node without children: not written, not used
         row_stats(p, 1, t, lane, m, z);
         if (lane == 0) {
           sh.mq[t] = m;
@@ -310,40 +362,49 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
     }
   }
   __syncthreads();
-
-  // Every node's children, a wave per node.
-  for (int t = wave; t < p.nodes; t += kWalkWaves) {
-    const uint16_t* rp = p.target + t * p.ldt;
-    const uint16_t* rq = drawn ? p.draft + t * p.ldd : nullptr;
-    double left = p.greedy ? 0.0 : sh.zp[t];           // point drafts: weight not yet rejected
-    int rejected = 0;
-    Residual r{0.0, 1.0, 0};
-    for (int s = t + 1; s < p.nodes; ++s) {
-      if (sh.parent[s] != t) continue;
-      const int x = sh.token[s];
-      const bool in = x >= 0 && x < p.vocab;
-      bool ok = false;
-      if (p.greedy) {
-        ok = x == sh.best[t];
-      } else if (!drawn) {
-        bool fresh = in;                               // a sibling's token that was rejected has no weight left
-        for (int b = t + 1; b < s && fresh; ++b) fresh = !(sh.parent[b] == t && sh.token[b] == x);
-        const double w = fresh ? weight(logit(rp, x), sh.mp[t], p.scale_log2) : 0.0;
-        ok = (double)p.accept_u[s] * left < w;
-        left = fmax(left - w, 0.0);
-      } else {
-        if (rejected == p.max_children) break;
-        const double pw = in ? weight(logit(rp, x), sh.mp[t], p.scale_log2) / sh.zp[t] : 0.0;
-        const double qw = in ? weight(logit(rq, x), sh.mq[t], p.scale_log2) / sh.zq[t] : 0.0;
-        ok = (double)p.accept_u[s] * qw * r.s < fmax(pw - r.a * qw, 0.0);
-        if (!ok) r = residual(p, t, rejected + 1, lane);
+  if (!p.greedy) {
+    for (int s = tid; s < p.nodes; s += kWalkThreads) {
+      const int t = sh.parent[s], x = sh.token[s];
+      double pw = 0.0, qw = 0.0;
+      if (t >= 0) {
+        pw = probability(p.target + t * p.ldt, x, p.vocab, make_scale(sh.mp[t], p.scale_log2), sh.zp[t]);
+        if (drawn)
+          qw = probability(p.draft + t * p.ldd, x, p.vocab, make_scale(sh.mq[t], p.scale_log2), sh.zq[t]);
+        else                                           // a sibling's token that was rejected has nothing left
+          for (int b = t + 1; b < s; ++b)
+            if (sh.parent[b] == t && sh.token[b] == x) pw = 0.0;
       }
-      if (ok) {
-        if (lane == 0) sh.next[t] = s;
-        break;
-      }
-      ++rejected;
+      sh.pw[s] = pw;
+      sh.qw[s] = qw;
     }
+    __syncthreads();
+  }
+
+  // Every node's children in order, a wave per node.
+  for (int t = wave; t < p.nodes; t += kWalkWaves) {
+    double left = 1.0;                                 // point drafts: what the rejected siblings leave
+    int rejected = 0, taken = -1;
+    Residual r{0.0, 1.0, 0};
+    for (int s0 = t + 1; s0 < p.nodes && taken < 0; s0 += 64) {
+      unsigned long long hits = __ballot(s0 + lane < p.nodes && sh.parent[min(s0 + lane, kNodes - 1)] == t);
+      for (; hits && taken < 0; hits &= hits - 1) {
+        const int s = s0 + __builtin_ctzll(hits);
+        bool ok;
+        if (p.greedy) {
+          ok = sh.token[s] == sh.best[t];
+        } else if (!drawn) {
+          ok = (double)sh.u[s] * left < sh.pw[s];
+          left = fmax(left - sh.pw[s], 0.0);
+        } else {
+          if (rejected == p.max_children) break;
+          ok = (double)sh.u[s] * sh.qw[s] * r.s < fmax(sh.pw[s] - r.a * sh.qw[s], 0.0);
+          if (!ok) reject(p, t, rejected + 1, lane, r);
+          ++rejected;
+        }
+        if (ok) taken = s;
+      }
+    }
+    if (lane == 0) sh.next[t] = taken;
   }
   __syncthreads();
 
@@ -351,145 +412,190 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
     int n = 0, t = 0;
     for (; t >= 0; t = sh.next[t]) sh.path[n++] = t;
     sh.count = n;
+    sh.first = 0x7fffffff;
+    sh.tail = -1;
+    sh.chunk = -1;
   }
   __syncthreads();
   const int count = sh.count, node = sh.path[count - 1];
 
+  int last = 0;
   if (p.greedy) {
-    if (tid == 0) sh.last = sh.best[node];
-    __syncthreads();
+    last = sh.best[node];
   } else {
-    // The last token: choose a chunk, then the index in it.  What is left of
-    // the distribution: chunk sums in a global array, or for point drafts
-    // computed again without the rejected tokens (subtracting their weights
-    // would leave rounding where nothing is left).
+    // The last token: choose a chunk by the chunks' sums of what is left of the distribution,
+    // then the index in it.
     const uint16_t* rp = p.target + node * p.ldt;
-    const float mp = sh.mp[node];
-    int children = 0;
-    for (int s = node + 1; s < p.nodes; ++s) children += sh.parent[s] == node;
+    const Scale sp = make_scale(sh.mp[node], p.scale_log2);
+    const double ip = 1.0 / sh.zp[node];
     Residual r{0.0, 1.0, 0};
-    if (drawn) r = residual(p, node, min(children, p.max_children), lane);
-    const double a = r.round ? r.a / sh.zq[node] : 0.0, ip = 1.0 / sh.zp[node];
+    int children = 0;
+    for (int s0 = node + 1; s0 < p.nodes; s0 += 64)
+      children += __builtin_popcountll(__ballot(s0 + lane < p.nodes && sh.parent[min(s0 + lane, kNodes - 1)] == node));
+    if (drawn)
+      for (int k = 1; k <= min(children, p.max_children); ++k) reject(p, node, k, lane, r);
+    const double a = r.round ? r.a / sh.zq[node] : 0.0;
     const uint16_t* rq = r.round ? p.draft + node * p.ldd : nullptr;
+    const Scale sq = make_scale(r.round ? sh.mq[node] : 0.0f, p.scale_log2);
     const double* rs = r.round ? p.rounds + ((long long)(r.round - 1) * p.nodes + node) * p.chunks : nullptr;
+    const bool holes = !drawn && children;             // rejected tokens of point drafts
 
-    auto mark = [&](int c) {                            // the chunk's rejected tokens
-      for (int i = tid; i < kVerifyChunk / 32; i += kWalkThreads) sh.gone[i] = 0u;
-      __syncthreads();
-      if (!drawn)
+    // This thread's eight of chunk c, without the rejected tokens.
+    auto chunk_weights = [&](int c, double (&w)[8]) {
+      if (holes) {
+        __syncthreads();                               // sh.gone may still be read
+        for (int i = tid; i < kMaxChunk / 32; i += kWalkThreads) sh.gone[i] = 0u;
+        __syncthreads();
         for (int s = node + 1 + tid; s < p.nodes; s += kWalkThreads) {
-          const int x = sh.token[s] - c * kVerifyChunk;
-          if (sh.parent[s] == node && sh.token[s] >= 0 && x >= 0 && x < kVerifyChunk) atomicOr(&sh.gone[x >> 5], 1u << (x & 31));
+          const int x = sh.token[s] - c * p.chunk;
+          if (sh.parent[s] == node && sh.token[s] >= 0 && x >= 0 && x < p.chunk) atomicOr(&sh.gone[x >> 5], 1u << (x & 31));
         }
-      __syncthreads();
-    };
-    auto weights = [&](int c, double (&w)[kPer]) {      // this thread's eight of chunk c
-      const int i0 = kPer * tid, v = c * kVerifyChunk + i0;
-      float x[8], y[8];
+        __syncthreads();
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = 0.0;
+      const int i0 = 8 * tid, v = c * p.chunk + i0;
+      if (i0 >= p.chunk || v >= p.vocab) return;
+      float x[8];
       load8(rp, v, p.vocab, x);
-      if (rq) load8(rq, v, p.vocab, y);
+      weights8(x, v, p.vocab, sp, w);
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        w[e] = 0.0;
-        if (v + e < p.vocab && !((sh.gone[(i0 + e) >> 5] >> ((i0 + e) & 31)) & 1u)) {
-          w[e] = weight(x[e], mp, p.scale_log2) * ip;
-          if (rq) w[e] = fmax(w[e] - weight(y[e], sh.mq[node], p.scale_log2) * a, 0.0);
-        }
+      for (int e = 0; e < 8; ++e) w[e] *= ip;
+      if (rq) {
+        float y[8];
+        double wq[8];
+        load8(rq, v, p.vocab, y);
+        weights8(y, v, p.vocab, sq, wq);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = fmax(w[e] - wq[e] * a, 0.0);
+      }
+      if (holes) {
+        const unsigned gone = (sh.gone[i0 >> 5] >> (i0 & 31)) & 0xffu;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = (gone >> e) & 1u ? 0.0 : w[e];
       }
     };
-    auto chunk_sum = [&](int c) -> double {
-      if (rs) return rs[c];
-      bool touched = false;
-      if (!drawn)
-        for (int s = node + 1; s < p.nodes; ++s)
-          touched |= sh.parent[s] == node && sh.token[s] >= 0 && sh.token[s] / kVerifyChunk == c;
-      if (!touched) return p.sums[(long long)node * p.chunks + c] * weight(p.maxes[(long long)node * p.chunks + c], mp, p.scale_log2) * ip;
-      double w[kPer];
-      mark(c);
-      weights(c, w);
-      double s = 0.0;
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) s += w[e];
-      return block_sum(s, sh);
-    };
-    double total = 0.0;
-    for (int c = 0; c < p.chunks; ++c) total += chunk_sum(c);
-    const double goal = (double)*p.sample_u * total;
-    double before = 0.0;
-    int chunk = -1;                                      // the first chunk whose end passes the goal, else the last with weight
-    double chunk_before = 0.0;
-    for (int c = 0; c < p.chunks; ++c) {
-      const double s = chunk_sum(c);
-      if (s > 0.0) {
-        chunk = c;
-        chunk_before = before;
+
+    // Chunk sums into global scratch (the node's own: nothing else reads it any more).  Point
+    // drafts: without the rejected tokens' weights, subtracted where enough is left that the
+    // rounding of the subtraction does not matter, else summed again.
+    double* sums = p.sums + (long long)node * p.chunks;
+    for (int c = tid; c < p.chunks; c += kWalkThreads) {
+      double s = rs ? rs[c] : sums[c] * weight(p.maxes[(long long)node * p.chunks + c], sp) * ip;
+      if (holes) {
+        const double all = s;
+        for (int k = node + 1; k < p.nodes; ++k)
+          if (sh.parent[k] == node && sh.token[k] >= 0 && sh.token[k] / p.chunk == c) s -= sh.pw[k];
+        if (s < 1e-3 * all) s = -1.0;                  // to be summed again
       }
-      before += s;
-      if (s > 0.0 && before > goal) break;
+      sums[c] = s;
     }
-    if (chunk < 0) {                                     // every child was rejected and nothing else has weight
-      if (tid == 0) sh.last = 0;
-    } else {
-      double w[kPer];
-      mark(chunk);
-      weights(chunk, w);
-      if (tid == 0) sh.last = -1;
+    __syncthreads();
+    if (holes)
+      for (int k = node + 1; k < p.nodes; ++k) {       // only these chunks can be marked
+        if (sh.parent[k] != node || sh.token[k] < 0 || sh.token[k] >= p.vocab) continue;
+        const int c = sh.token[k] / p.chunk;
+        if (sums[c] >= 0.0) continue;                  // uniform: nothing is written between the barriers
+        double w[8];
+        chunk_weights(c, w);
+        const double s = block_sum(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])), sh);
+        if (tid == 0) sums[c] = s;
+        __syncthreads();
+      }
+    // Wave 0: the total, then the first chunk whose end passes the goal, else the last with weight.
+    if (wave == 0) {
+      double total = 0.0;
+      for (int c = lane; c < p.chunks; c += 64) total += sums[c];
+      total = wave_sum(total);
+      const double goal = (double)sample_u * total;
+      double before = 0.0, chunk_before = 0.0;
+      int chunk = -1;
+      bool passed = false;
+      for (int c0 = 0; c0 < p.chunks && !passed; c0 += 64) {
+        const double s = c0 + lane < p.chunks ? sums[c0 + lane] : 0.0;
+        double end = s;                                // inclusive scan
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+          const double y = __shfl_up(end, d);
+          if (lane >= d) end += y;
+        }
+        const unsigned long long some = __ballot(s > 0.0), past = __ballot(s > 0.0 && before + end > goal);
+        if (some) {
+          const int at = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+          chunk = c0 + at;
+          chunk_before = before + __shfl(end - s, at);
+          passed = past != 0;
+        }
+        before += __shfl(end, 63);
+      }
+      if (lane == 0) {
+        sh.chunk = chunk;
+        sh.before = chunk_before;
+        sh.total = total;
+      }
+    }
+    __syncthreads();
+    const int chunk = sh.chunk;
+    if (chunk >= 0) {                                  // else all is rejected and nothing has weight: token 0
+      const double goal = (double)sample_u * sh.total;
+      double w[8];
+      chunk_weights(chunk, w);
       double run = 0.0;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) run += w[e];
-      double incl = run;                                 // inclusive scan over the wave, then over the waves
+      for (int e = 0; e < 8; ++e) run += w[e];
+      double end = run;                                // inclusive scan over the wave, then over the waves
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
-        const double y = __shfl_up(incl, d);
-        if (lane >= d) incl += y;
+        const double y = __shfl_up(end, d);
+        if (lane >= d) end += y;
       }
+      __syncthreads();                                 // sh.wave may still be read
+      if (lane == 63) sh.wave[wave] = end;
       __syncthreads();
-      if (lane == 63) sh.wave[wave] = incl;
-      __syncthreads();
-      double base = chunk_before;
-      for (int i = 0; i < wave; ++i) base += sh.wave[i];
-      double cum = base + (incl - run);
+      double cum = sh.before + (end - run);
+      for (int i = 0; i < wave; ++i) cum += sh.wave[i];
       int hit = 0x7fffffff, tail = -1;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) {
+      for (int e = 0; e < 8; ++e) {
         cum += w[e];
         if (w[e] > 0.0) {
-          tail = kPer * tid + e;
-          if (cum > goal && hit == 0x7fffffff) hit = kPer * tid + e;
+          tail = 8 * tid + e;
+          if (cum > goal && hit == 0x7fffffff) hit = 8 * tid + e;
         }
       }
-      __shared__ int first, final_;
-      if (tid == 0) {
-        first = 0x7fffffff;
-        final_ = -1;
-      }
+      if (hit != 0x7fffffff) atomicMin(&sh.first, hit);
+      if (tail >= 0) atomicMax(&sh.tail, tail);
       __syncthreads();
-      if (hit != 0x7fffffff) atomicMin(&first, hit);
-      if (tail >= 0) atomicMax(&final_, tail);
-      __syncthreads();
-      if (tid == 0) sh.last = chunk * kVerifyChunk + (first != 0x7fffffff ? first : max(final_, 0));
+      last = chunk * p.chunk + (sh.first != 0x7fffffff ? sh.first : max(sh.tail, 0));
     }
-    __syncthreads();
   }
 
   for (int i = tid; i < p.nodes; i += kWalkThreads) {
     p.path[i] = i < count ? sh.path[i] : -1;
-    p.emitted[i] = i < count - 1 ? sh.token[sh.path[i + 1]] : i == count - 1 ? sh.last : -1;
+    p.emitted[i] = i < count - 1 ? sh.token[sh.path[i + 1]] : i == count - 1 ? last : -1;
   }
   if (tid == 0) *p.count = count;
+}
+
+template <int kRuns>
+void launch_passes(const TreeVerifyParams& p, hipStream_t stream) {
+  if (p.greedy) {
+    hipLaunchKernelGGL(verify_argmax_kernel<kRuns>, dim3(p.chunks, p.nodes), dim3(kThreads), 0, stream, p);
+    return;
+  }
+  hipLaunchKernelGGL(verify_stats_kernel<kRuns>, dim3(p.chunks, p.nodes, p.draft ? 2 : 1), dim3(kThreads), 0, stream, p);
+  if (p.draft)
+    for (int r = 1; r <= p.max_children; ++r)
+      hipLaunchKernelGGL(verify_round_kernel<kRuns>, dim3(p.chunks, p.nodes), dim3(kThreads), 0, stream, p, r);
 }
 
 }  // namespace
 
 hipError_t launch_tree_verify(const TreeVerifyParams& p, hipStream_t stream) {
-  if (p.greedy) {
-    hipLaunchKernelGGL(verify_argmax_kernel, dim3(p.chunks, p.nodes), dim3(kThreads), 0, stream, p);
-  } else {
-    hipLaunchKernelGGL(verify_stats_kernel, dim3(p.chunks, p.nodes, p.draft ? 2 : 1), dim3(kThreads), 0, stream, p);
-    if (p.draft)
-      for (int r = 1; r <= p.max_children; ++r)
-        hipLaunchKernelGGL(verify_round_kernel, dim3(p.chunks, p.nodes), dim3(kThreads), 0, stream, p, r);
-  }
+  if (p.chunk == 8 * kThreads * 4)
+    launch_passes<4>(p, stream);
+  else
+    launch_passes<1>(p, stream);
   hipLaunchKernelGGL(verify_walk_kernel, dim3(1), dim3(kWalkThreads), 0, stream, p);
   return hipGetLastError();
 }
