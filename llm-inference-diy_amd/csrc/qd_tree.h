@@ -64,10 +64,19 @@ struct TreeAttnPlan {
 };
 
 // max_splits: what the workspace is sized for, at any prefix.
+//
+// Block rows: the smallest of 16, 32 and 64 that holds all query rows, else 128-row blocks
+// unless 64-row blocks leave fewer rows empty (192 rows, 32 query heads on 8 cache heads over
+// 16001 rows: 32.4 us in 64-row blocks, 33.7 in 128-row ones).
+// Splits: at most one workgroup per CU, and no more than the rounds need: a key wave takes a
+// tile per round, and every further split adds partials to write and fold (16 cache heads, 64
+// nodes over 4096 rows, 3 rounds: 18.6 us at 12 splits, 19.5 at 16; 27 nodes over 4096 rows,
+// 2 rounds: 13.3 at 9, 14.0 at 16).  One split, without the second launch, where its rounds
+// cost no more than that launch (5 nodes over 512 rows, 3 rounds: 7.6 against 7.9 us, and one
+// launch less for the host; over 1024 rows, 5 rounds: 9.1 against 8.3).
 inline TreeAttnPlan tree_attn_plan(int nodes, int heads, int kv_heads, int prefix, int num_cus, int* max_splits) {
   TreeAttnPlan plan;
   const int rows = nodes * (heads / kv_heads);
-  // 128-row blocks unless 64-row blocks leave fewer rows empty
   const bool wide = (rows + 127) / 128 * 2 == (rows + 63) / 64;
   plan.block_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : wide ? 128 : 64;
   plan.key_waves = rows <= 32 ? 8 : wide ? 2 : 4;
@@ -75,9 +84,13 @@ inline TreeAttnPlan tree_attn_plan(int nodes, int heads, int kv_heads, int prefi
   const int most = num_cus / (plan.blocks * kv_heads);
   *max_splits = most < 1 ? 1 : most;
   const int tiles = (prefix + 31) / 32 + (nodes + 31) / 32;
-  const int by_tiles = (tiles + plan.key_waves - 1) / plan.key_waves;
-  plan.splits = *max_splits < by_tiles ? *max_splits : by_tiles;
-  plan.rounds = (by_tiles + plan.splits - 1) / plan.splits;
+  const int groups = (tiles + plan.key_waves - 1) / plan.key_waves;   // rounds of one split
+  plan.rounds = (groups + *max_splits - 1) / *max_splits;
+  plan.splits = (groups + plan.rounds - 1) / plan.rounds;
+  if (groups <= (plan.key_waves == 8 ? 3 : 2)) {
+    plan.splits = 1;
+    plan.rounds = groups;
+  }
   return plan;
 }
 hipError_t launch_tree_attention(const TreeAttnParams& p, const TreeAttnPlan& plan, hipStream_t stream);

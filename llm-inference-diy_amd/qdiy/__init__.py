@@ -212,29 +212,36 @@ def _ptr(t: torch.Tensor, name: str, contiguous: bool = True) -> int:
     raise ValueError(f"{name} must be contiguous")
 
 
-def _typed_ptr(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int) -> int:
-    """The address of a contiguous GPU tensor of `dtype` with at least `numel` elements."""
-    if not isinstance(t, _Tensor) or t.dtype is not dtype:
-        raise TypeError(f"{name} must be a {dtype} torch.Tensor")
-    if not t.is_cuda or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous GPU tensor")
-    if t.numel() < numel:
-        raise ValueError(f"{name} holds {t.numel()} elements, needs {numel}")
-    return t.data_ptr()
+def _arg(t: torch.Tensor, name: str, dtype: torch.dtype, dev: int, numel: int) -> int:
+    """The address of a contiguous tensor of `dtype` on GPU `dev` (the current device, on which
+    kernels run) with at least `numel` elements."""
+    try:
+        if t.dtype is dtype and t.get_device() == dev and t.numel() >= numel and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        raise TypeError(f"{name} must be a torch.Tensor") from None
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{dev}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    raise ValueError(f"{name} holds {t.numel()} elements, needs {numel}")
 
 
-def _workspace(t: torch.Tensor) -> tuple:
-    if not isinstance(t, _Tensor) or not t.is_cuda or not t.is_contiguous():
-        raise TypeError("workspace must be a contiguous GPU tensor")
-    return t.data_ptr(), t.numel() * t.element_size()
+def _workspace(t: torch.Tensor, dev: int) -> tuple:
+    if not isinstance(t, _Tensor) or not t.is_contiguous():
+        raise TypeError("workspace must be a contiguous tensor")
+    if t.get_device() != dev:
+        raise ValueError(f"workspace is on {t.device}, the current device is cuda:{dev}")
+    return t.data_ptr(), t.nbytes
 
 
-def _on_one_device(*tensors) -> None:
-    """Kernels run on the current device: tensors of another one are refused."""
-    dev = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"a tensor is on device {t.get_device()}, the current device is {dev}")
+def _current_device() -> int:
+    try:
+        return torch._C._cuda_getDevice()
+    except AttributeError:
+        return torch.cuda.current_device()
 
 
 class Context:
@@ -456,10 +463,9 @@ class Context:
                                              HEAD_DIM, _stream(stream)))
 
     # -- trees of drafted tokens -------------------------------------------------
-    def _check_rows(self, t: torch.Tensor, name: str, rows: int, row: int, head: int, base: int = 0) -> None:
-        last = base + (rows - 1) * row + (self.num_heads - 1) * head + HEAD_DIM
-        if rows >= 1 and t.numel() < last:
-            raise ValueError(f"{name} holds {t.numel()} elements; {rows} rows need {last}")
+    def _span(self, rows: int, row: int, head: int, base: int = 0) -> int:
+        """Elements that `rows` rows of the cache's heads reach at these strides."""
+        return base + (rows - 1) * row + (self.num_heads - 1) * head + HEAD_DIM if rows >= 1 else 0
 
     def tree_qkv_rope(self, qkv: torch.Tensor, bias, depth: torch.Tensor, q_out: torch.Tensor,
                       k_tree: torch.Tensor, v_tree: torch.Tensor, prefix: int, nodes: int,
@@ -468,24 +474,21 @@ class Context:
                       tree_head_stride: int = HEAD_DIM, stream=None) -> None:
         """qd_tree_qkv_rope: bias and RoPE of a drafted tree's nodes at prefix + depth; the
         rotated Q rows into q_out, the nodes' K/V rows into k_tree and v_tree."""
-        H, KH = self.num_heads if num_heads is None else num_heads, self.num_heads
+        KH = self.num_heads
+        H = KH if num_heads is None else num_heads
         row = (H + 2 * KH) * HEAD_DIM
         qkv_stride = row if qkv_stride is None else qkv_stride
         q_stride = H * HEAD_DIM if q_stride is None else q_stride
         tree_row_stride = KH * HEAD_DIM if tree_row_stride is None else tree_row_stride
-        if qkv.numel() < (nodes - 1) * qkv_stride + row or q_out.numel() < (nodes - 1) * q_stride + H * HEAD_DIM:
-            raise ValueError("qkv or q_out too small for nodes, num_heads and the strides")
-        if bias is not None and bias.numel() < row:
-            raise ValueError(f"bias needs {row} elements")
-        self._check_rows(k_tree, "k_tree", nodes, tree_row_stride, tree_head_stride)
-        self._check_rows(v_tree, "v_tree", nodes, tree_row_stride, tree_head_stride)
-        _on_one_device(qkv, bias, depth, q_out, k_tree, v_tree)
-        _check(load().qd_tree_qkv_rope(self._h, _ptr(qkv, "qkv"), qkv_stride,
-                                       None if bias is None else _ptr(bias, "bias"),
-                                       _typed_ptr(depth, "depth", torch.int32, nodes), _ptr(q_out, "q_out"),
-                                       q_stride, _ptr(k_tree, "k_tree"), _ptr(v_tree, "v_tree"),
-                                       tree_row_stride, tree_head_stride, prefix, nodes, H, HEAD_DIM,
-                                       _stream(stream)))
+        span = self._span(nodes, tree_row_stride, tree_head_stride)
+        dev = _current_device()
+        _check(load().qd_tree_qkv_rope(
+            self._h, _arg(qkv, "qkv", _F16, dev, (nodes - 1) * qkv_stride + row), qkv_stride,
+            None if bias is None else _arg(bias, "bias", _F16, dev, row),
+            _arg(depth, "depth", torch.int32, dev, nodes),
+            _arg(q_out, "q_out", _F16, dev, (nodes - 1) * q_stride + H * HEAD_DIM), q_stride,
+            _arg(k_tree, "k_tree", _F16, dev, span), _arg(v_tree, "v_tree", _F16, dev, span), tree_row_stride,
+            tree_head_stride, prefix, nodes, H, HEAD_DIM, _stream(stream)))
 
     def tree_attention_workspace_bytes(self, nodes: int, num_heads: int | None = None) -> int:
         """qd_tree_attention_workspace_bytes: enough at any prefix."""
@@ -502,26 +505,23 @@ class Context:
                        stream=None) -> torch.Tensor:
         """qd_tree_attention: node t of a drafted tree attends over the cache rows [0, prefix)
         and the node rows whose bit is set in row t of mask (int64 words)."""
-        H, KH = self.num_heads if num_heads is None else num_heads, self.num_heads
+        KH = self.num_heads
+        H = KH if num_heads is None else num_heads
         row = H * HEAD_DIM
         q_stride = row if q_stride is None else q_stride
         out_stride = row if out_stride is None else out_stride
         tree_row_stride = KH * HEAD_DIM if tree_row_stride is None else tree_row_stride
-        if q.numel() < (nodes - 1) * q_stride + row or out.numel() < (nodes - 1) * out_stride + row:
-            raise ValueError("q and out need (nodes-1)*stride + num_heads*128 elements")
-        if 0 <= prefix <= self.max_seqlen:
-            self._check_rows(k_layer, "k_layer", prefix, self.kv_row_stride, self.kv_head_stride)
-            self._check_rows(v_layer, "v_layer", prefix, self.kv_row_stride, self.kv_head_stride)
-        self._check_rows(k_tree, "k_tree", nodes, tree_row_stride, tree_head_stride)
-        self._check_rows(v_tree, "v_tree", nodes, tree_row_stride, tree_head_stride)
-        _on_one_device(q, k_layer, v_layer, k_tree, v_tree, mask, out, workspace)
-        ws, ws_bytes = _workspace(workspace)
-        _check(load().qd_tree_attention(self._h, _ptr(q, "q"), q_stride, _ptr(k_layer, "k_layer"),
-                                        _ptr(v_layer, "v_layer"), _ptr(k_tree, "k_tree"), _ptr(v_tree, "v_tree"),
-                                        tree_row_stride, tree_head_stride,
-                                        _typed_ptr(mask, "mask", torch.int64, nodes * ((nodes + 63) // 64)),
-                                        _ptr(out, "out"), out_stride, prefix, nodes, H, HEAD_DIM, ws, ws_bytes,
-                                        _stream(stream)))
+        cache = self._span(min(prefix, self.max_seqlen), self.kv_row_stride, self.kv_head_stride)
+        span = self._span(nodes, tree_row_stride, tree_head_stride)
+        dev = _current_device()
+        ws, ws_bytes = _workspace(workspace, dev)
+        _check(load().qd_tree_attention(
+            self._h, _arg(q, "q", _F16, dev, (nodes - 1) * q_stride + row), q_stride,
+            _arg(k_layer, "k_layer", _F16, dev, cache), _arg(v_layer, "v_layer", _F16, dev, cache),
+            _arg(k_tree, "k_tree", _F16, dev, span), _arg(v_tree, "v_tree", _F16, dev, span), tree_row_stride,
+            tree_head_stride, _arg(mask, "mask", torch.int64, dev, nodes * ((nodes + 63) // 64)),
+            _arg(out, "out", _F16, dev, (nodes - 1) * out_stride + row), out_stride, prefix, nodes, H, HEAD_DIM,
+            ws, ws_bytes, _stream(stream)))
         return out
 
     def tree_commit(self, k_tree: torch.Tensor, v_tree: torch.Tensor, k_cache: torch.Tensor,
@@ -533,24 +533,25 @@ class Context:
         layers.  Layers are numel // layers elements apart by default."""
         if layers < 1:
             raise ValueError("layers must be >= 1")
+        if tree_layer_stride is None:
+            if v_tree.numel() != k_tree.numel():
+                raise ValueError("k_tree and v_tree differ in size: give tree_layer_stride")
+            tree_layer_stride = k_tree.numel() // layers
+        if cache_layer_stride is None:
+            if v_cache.numel() != k_cache.numel():
+                raise ValueError("k_cache and v_cache differ in size: give cache_layer_stride")
+            cache_layer_stride = k_cache.numel() // layers
         tree_row_stride = self.num_heads * HEAD_DIM if tree_row_stride is None else tree_row_stride
-        tl = k_tree.numel() // layers if tree_layer_stride is None else tree_layer_stride
-        cl = k_cache.numel() // layers if cache_layer_stride is None else cache_layer_stride
-        if tree_layer_stride is None and v_tree.numel() != k_tree.numel():
-            raise ValueError("k_tree and v_tree differ in size: give tree_layer_stride")
-        if cache_layer_stride is None and v_cache.numel() != k_cache.numel():
-            raise ValueError("k_cache and v_cache differ in size: give cache_layer_stride")
-        for t, name in ((k_tree, "k_tree"), (v_tree, "v_tree")):
-            self._check_rows(t, name, nodes, tree_row_stride, tree_head_stride, (layers - 1) * tl)
-        for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-            self._check_rows(t, name, min(self.max_seqlen, max(0, prefix) + nodes), self.kv_row_stride,
-                             self.kv_head_stride, (layers - 1) * cl)
-        _on_one_device(k_tree, v_tree, k_cache, v_cache, path, count)
-        _check(load().qd_tree_commit(self._h, _ptr(k_tree, "k_tree", False), _ptr(v_tree, "v_tree", False), tl,
-                                     tree_row_stride, tree_head_stride, _ptr(k_cache, "k_cache"),
-                                     _ptr(v_cache, "v_cache"), cl, _typed_ptr(path, "path", torch.int32, nodes),
-                                     _typed_ptr(count, "count", torch.int32, 1), prefix, nodes, layers,
-                                     _stream(stream)))
+        span = self._span(nodes, tree_row_stride, tree_head_stride, (layers - 1) * tree_layer_stride)
+        cache = self._span(min(self.max_seqlen, prefix + nodes), self.kv_row_stride, self.kv_head_stride,
+                           (layers - 1) * cache_layer_stride)
+        dev = _current_device()
+        _check(load().qd_tree_commit(
+            self._h, _arg(k_tree, "k_tree", _F16, dev, span), _arg(v_tree, "v_tree", _F16, dev, span),
+            tree_layer_stride, tree_row_stride, tree_head_stride, _arg(k_cache, "k_cache", _F16, dev, cache),
+            _arg(v_cache, "v_cache", _F16, dev, cache), cache_layer_stride,
+            _arg(path, "path", torch.int32, dev, nodes), _arg(count, "count", torch.int32, dev, 1), prefix, nodes,
+            layers, _stream(stream)))
 
 
 def xcd_placement(count: int = 256) -> list:
@@ -683,21 +684,17 @@ def tree_verify(target_logits: torch.Tensor, tokens: torch.Tensor, parents: torc
     token after it; greedy at temperature 0, else from the given uniforms accept_u and sample_u."""
     ldt = vocab if ldt is None else ldt
     ldd = vocab if ldd is None else ldd
-    if target_logits.numel() < (nodes - 1) * ldt + vocab:
-        raise ValueError("target_logits too small for nodes, vocab and ldt")
-    if draft_logits is not None and draft_logits.numel() < (nodes - 1) * ldd + vocab:
-        raise ValueError("draft_logits too small for nodes, vocab and ldd")
-    _on_one_device(target_logits, draft_logits, tokens, parents, accept_u, sample_u, workspace, path, emitted, count)
-    ws, ws_bytes = _workspace(workspace)
+    dev = _current_device()
     i32, f32 = torch.int32, torch.float32
+    ws, ws_bytes = _workspace(workspace, dev)
     _check(load().qd_tree_verify(
-        _ptr(target_logits, "target_logits"), ldt,
-        None if draft_logits is None else _ptr(draft_logits, "draft_logits"), ldd,
-        _typed_ptr(tokens, "tokens", i32, nodes), _typed_ptr(parents, "parents", i32, nodes),
-        None if accept_u is None else _typed_ptr(accept_u, "accept_u", f32, nodes),
-        None if sample_u is None else _typed_ptr(sample_u, "sample_u", f32, 1), temperature, nodes, vocab,
-        max_children, ws, ws_bytes, _typed_ptr(path, "path", i32, nodes),
-        _typed_ptr(emitted, "emitted", i32, nodes), _typed_ptr(count, "count", i32, 1), _stream(stream)))
+        _arg(target_logits, "target_logits", _F16, dev, (nodes - 1) * ldt + vocab), ldt,
+        None if draft_logits is None else _arg(draft_logits, "draft_logits", _F16, dev, (nodes - 1) * ldd + vocab), ldd,
+        _arg(tokens, "tokens", i32, dev, nodes), _arg(parents, "parents", i32, dev, nodes),
+        None if accept_u is None else _arg(accept_u, "accept_u", f32, dev, nodes),
+        None if sample_u is None else _arg(sample_u, "sample_u", f32, dev, 1), temperature, nodes, vocab,
+        max_children, ws, ws_bytes, _arg(path, "path", i32, dev, nodes), _arg(emitted, "emitted", i32, dev, nodes),
+        _arg(count, "count", i32, dev, 1), _stream(stream)))
 
 
 # ---------------------------------------------------------------- engine.h
