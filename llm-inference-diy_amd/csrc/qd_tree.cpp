@@ -188,10 +188,11 @@ int qd_tree_attention(qd_ctx* ctx, const uint16_t* q, long long q_stride, const 
 
 size_t qd_tree_verify_workspace_bytes(int nodes, int vocab, int max_children) {
   if (!verify_args_ok(nodes, vocab, max_children)) return 0;
-  const int chunk = qd::verify_chunk(nodes, vocab);
-  const size_t rows = (size_t)nodes * ((vocab + chunk - 1) / chunk);
-  return round16(2 * rows * sizeof(double)) + round16((size_t)max_children * rows * sizeof(double)) +
-         round16(2 * rows * sizeof(float)) + round16(rows * sizeof(int));
+  const size_t chunks = (vocab + qd::kVerifyChunk - 1) / qd::kVerifyChunk, runs = qd::verify_runs(nodes, (int)chunks);
+  const size_t rows = (size_t)nodes * chunks, groups = (size_t)nodes * ((chunks + runs - 1) / runs);
+  return round16(2 * rows * sizeof(double)) + round16(2 * groups * sizeof(double)) +
+         round16((size_t)max_children * rows * sizeof(double)) + round16(2 * groups * sizeof(float)) +
+         round16(groups * sizeof(int));
 }
 
 int qd_tree_verify(const uint16_t* target_logits, long long ldt, const uint16_t* draft_logits, long long ldd,
@@ -247,22 +248,26 @@ int qd_tree_verify(const uint16_t* target_logits, long long ldt, const uint16_t*
   p.count = count;
   p.ldt = ldt;
   p.ldd = drawn ? ldd : 0;
-  p.scale_log2 = greedy ? 0.0 : 1.4426950408889634 / (double)temperature;
+  p.scale_log2 = greedy ? 0.0 : 32.0 * 1.4426950408889634 / (double)temperature;
   p.nodes = nodes;
   p.vocab = vocab;
-  p.chunk = qd::verify_chunk(nodes, vocab);
-  p.chunks = (vocab + p.chunk - 1) / p.chunk;
+  p.chunks = (vocab + qd::kVerifyChunk - 1) / qd::kVerifyChunk;
+  p.runs = qd::verify_runs(nodes, p.chunks);
+  p.groups = (p.chunks + p.runs - 1) / p.runs;
   p.max_children = nodes > 1 ? max_children : 0;
   p.greedy = greedy;
-  const size_t rows = (size_t)nodes * p.chunks;
+  const size_t rows = (size_t)nodes * p.chunks, groups = (size_t)nodes * p.groups;
   char* ws = static_cast<char*>(workspace);
-  p.sums = reinterpret_cast<double*>(ws);
-  ws += round16(2 * rows * sizeof(double));
-  p.rounds = reinterpret_cast<double*>(ws);
-  ws += round16((size_t)max_children * rows * sizeof(double));
-  p.maxes = reinterpret_cast<float*>(ws);
-  ws += round16(2 * rows * sizeof(float));
-  p.args = reinterpret_cast<int*>(ws);
+  auto take = [&ws](size_t bytes) {
+    char* at = ws;
+    ws += round16(bytes);
+    return at;
+  };
+  p.sums = reinterpret_cast<double*>(take(2 * rows * sizeof(double)));
+  p.group_sums = reinterpret_cast<double*>(take(2 * groups * sizeof(double)));
+  p.rounds = reinterpret_cast<double*>(take((size_t)max_children * rows * sizeof(double)));
+  p.maxes = reinterpret_cast<float*>(take(2 * groups * sizeof(float)));
+  p.args = reinterpret_cast<int*>(take(groups * sizeof(int)));
   const hipError_t e = qd::launch_tree_verify(p, stream);
   return e == hipSuccess ? QD_OK : hip_fail(e, "tree verification launch");
 }

@@ -95,9 +95,11 @@ inline TreeAttnPlan tree_attn_plan(int nodes, int heads, int kv_heads, int prefi
 }
 hipError_t launch_tree_attention(const TreeAttnParams& p, const TreeAttnPlan& plan, hipStream_t stream);
 
-// Logits of a row per workgroup of the verification's passes over them: 8192, or 2048 where
-// that leaves the chip's CUs half empty.
-inline int verify_chunk(int nodes, int vocab) { return (long long)nodes * ((vocab + 8191) / 8192) >= 512 ? 8192 : 2048; }
+// Logits of a row per chunk of the verification's passes, and chunks per workgroup: 4, or 1 where
+// that would be fewer than two workgroups per CU (5 rows of 151936 logits: the argmax pass 3.8
+// us against 5.8).
+constexpr int kVerifyChunk = 2048;
+inline int verify_runs(int nodes, int chunks) { return (long long)nodes * ((chunks + 3) / 4) >= 512 ? 4 : 1; }
 
 struct TreeVerifyParams {
   const uint16_t* target;   // [nodes][vocab]
@@ -109,16 +111,17 @@ struct TreeVerifyParams {
   int* path;
   int* emitted;
   int* count;
-  // Workspace: per side (target, draft), node and chunk the largest logit and
-  // the chunk's sum of weights relative to it (greedy: the argmax and its
-  // logit); then per round, node and chunk the sums of max(p - A q, 0).
+  // Workspace.  A group is the chunks of one workgroup; per side (target, draft), node and group
+  // the largest logit and the sum of weights relative to it (greedy: the argmax and its logit),
+  // per chunk its part of that sum; then per round, node and chunk the sums of max(p - A q, 0).
   double* sums;             // [2][nodes][chunks]
+  double* group_sums;       // [2][nodes][groups]
   double* rounds;           // [max_children][nodes][chunks]
-  float* maxes;             // [2][nodes][chunks]
-  int* args;                // [nodes][chunks]
+  float* maxes;             // [2][nodes][groups]
+  int* args;                // [nodes][groups]
   long long ldt, ldd;
-  double scale_log2;        // log2(e) / temperature
-  int nodes, vocab, chunk, chunks, max_children;
+  double scale_log2;        // 32 log2(e) / temperature
+  int nodes, vocab, chunks, runs, groups, max_children;   // groups: workgroups per row
   int greedy;
 };
 hipError_t launch_tree_verify(const TreeVerifyParams& p, hipStream_t stream);

@@ -30,45 +30,73 @@ namespace {
 typedef _Float16 f16x8u __attribute__((ext_vector_type(8), aligned(2)));   // rows need not be 16-byte aligned
 
 constexpr int kNodes = QD_TREE_MAX_NODES;
-constexpr int kThreads = 256;                          // of the passes over chunks: runs of 8 logits per thread
+constexpr int kThreads = 256;                          // of the passes over chunks: 8 logits per thread and chunk
+static_assert(kVerifyChunk == 8 * kThreads, "a chunk is one run of 8 logits per thread");
 
-// Weight of a logit in a row (or chunk): `m` its largest logit, `scale` log2(e) / temperature.
+// Touches the argument block's cache lines at once: on its own the compiler loads each argument
+// where it is first used, and waits for a line each time.
+__device__ __forceinline__ void load_arguments(const TreeVerifyParams& p) {
+  static_assert(sizeof(TreeVerifyParams) > 128 && sizeof(TreeVerifyParams) <= 192, "three 64-byte lines");
+  asm volatile("" ::"s"(p.target), "s"(p.sums), "s"(p.groups));
+}
+
+// Weight of a logit in a row (or chunk): `m` its largest logit, `scale` 32 log2(e) / temperature
+// (exponents are counted in 32nds).
 struct Scale {
   float m;
   double md, scale;
 };
 __device__ __forceinline__ Scale make_scale(float m, double scale) { return Scale{m, (double)m, scale}; }
 
-// 2^x, x = (l - m) * scale <= 0, to a relative 1e-12: 2^n times the series of 2^f to degree 10 on
-// |f| <= 1/2 (remainder (ln2/2)^11 / 11! = 2e-13; the difference of two halves is exact).
-// Rounding to n by adding 1.5 * 2^52 leaves n in the low word, and adding n to the exponent
-// field scales: conversions, v_rndne_f64 and v_ldexp_f64 issue at a quarter of the rate of
-// v_fma_f64.  Below 2^-1000: 0, as for NaN (fmax drops it).  m is finite.
-__device__ __forceinline__ double weight_finite(float l, const Scale& s) {
-  const double x = fmax(((double)l - s.md) * s.scale, -1020.0);
+// 2^(j / 32).
+__device__ const double kPow32[32] = {
+    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
+    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
+    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
+    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
+    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0,
+};
+// Each workgroup's copy, 256 bytes: one entry per pair of LDS banks, so lanes never conflict.
+__device__ __forceinline__ void load_table(double* table) {
+  if (threadIdx.x < 32) table[threadIdx.x] = kPow32[threadIdx.x];
+}
+
+// 2^(x / 32), x = (l - m) * scale <= 0, to a relative 2e-12: 2^n 2^(j/32) times the series of
+// 2^(f/32) to degree 4 on |f| <= 1/2 (remainder (ln2/64)^5 / 5! = 1.3e-12; the difference of two
+// halves is exact).  Rounding to 32 n + j by adding 1.5 * 2^52 leaves it in the low word, and
+// adding n to the exponent field scales: the stats pass is bound by fp64 instructions, of
+// which this takes 11 (a series on |f| <= 1/2 of a whole exponent takes 18, and the pass over 64
+// rows of 151936 logits 13.0 us instead of KSTATS).  Below 2^-1000: 0, as for NaN (fmaxf drops
+// it).  m is finite.
+__device__ __forceinline__ double weight_finite(float l, const Scale& s, const double* table) {
+  const double x = ((double)l - s.md) * s.scale;
   const double t = x + 0x1.8p52;
   const double f = x - (t - 0x1.8p52);
-  double r = 7.054911620801121e-09;                    // ln2^k / k!, k = 10 .. 0
-  r = __builtin_fma(r, f, 1.0178086009239699e-07);
-  r = __builtin_fma(r, f, 1.3215486790144307e-06);
-  r = __builtin_fma(r, f, 1.5252733804059838e-05);
-  r = __builtin_fma(r, f, 0.00015403530393381608);
-  r = __builtin_fma(r, f, 0.0013333558146428441);
-  r = __builtin_fma(r, f, 0.009618129107628477);
-  r = __builtin_fma(r, f, 0.05550410866482158);
-  r = __builtin_fma(r, f, 0.2402265069591007);
-  r = __builtin_fma(r, f, 0.6931471805599453);
-  r = __builtin_fma(r, f, 1.0);
-  const long long bits = __builtin_bit_cast(long long, r);
-  const int lo = (int)bits, hi = (int)(bits >> 32) + ((int)__builtin_bit_cast(long long, t) << 20);
+  const int n = (int)__builtin_bit_cast(long long, t);
+  double r = 9.172562701824643e-09;                    // (ln2 / 32)^k / k!, k = 4 .. 1
+  r = __builtin_fma(r, f, 1.6938509724371819e-06);
+  r = __builtin_fma(r, f, 0.00023459619820224677);
+  r = __builtin_fma(r, f, 0.02166084939249829);
+  const double base = table[n & 31];
+  const long long bits = __builtin_bit_cast(long long, __builtin_fma(base, r * f, base));
+  const int lo = (int)bits, hi = (int)(bits >> 32) + ((n >> 5) << 20);
   const double w = __builtin_bit_cast(double, ((long long)hi << 32) | (unsigned)lo);
-  return x > -1000.0 ? w : 0.0;
+  return x > -32000.0 ? w : 0.0;                       // and where x is NaN
 }
 // The same for any m: the largest logits weigh 1 also where they are infinite.
-__device__ __forceinline__ double weight(float l, const Scale& s) {
-  if (fabsf(s.m) < __builtin_inff()) return weight_finite(l, s);
+__device__ __forceinline__ double weight(float l, const Scale& s, const double* table) {
+  if (fabsf(s.m) < __builtin_inff()) return weight_finite(l, s, table);
   if (l != l) l = -__builtin_inff();
   return l == s.m ? 1.0 : 0.0;
+}
+
+// The same as a function of its own, for the one-workgroup kernel: its time is that of fetching
+// instructions that run once, and an inlined weight is 40 of them.
+__device__ __attribute__((noinline)) double weight_call(float l, float m, double scale, const double* table) {
+  return weight(l, make_scale(m, scale), table);
 }
 
 __device__ __forceinline__ double wave_sum(double x) {
@@ -90,59 +118,68 @@ __device__ __forceinline__ void load8(const uint16_t* row, int v, int vocab, flo
   }
 }
 // Their weights; 0 past the row's end.
-__device__ __forceinline__ void weights8(const float (&x)[8], int v, int vocab, const Scale& s, double (&w)[8]) {
+__device__ __forceinline__ void weights8(const float (&x)[8], int v, int vocab, const Scale& s, const double* table,
+                                         double (&w)[8]) {
   if (fabsf(s.m) < __builtin_inff()) {                 // uniform over a chunk
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = weight_finite(x[e], s);
+    for (int e = 0; e < 8; ++e) w[e] = weight_finite(x[e], s, table);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = v + e < vocab ? weight(x[e], s) : 0.0;
+    for (int e = 0; e < 8; ++e) w[e] = v + e < vocab ? weight(x[e], s, table) : 0.0;
   }
 }
 
-// (1) Sampled: blockIdx = (chunk, node, side), a chunk kRuns runs per thread.  The drafter's
-// rows of nodes without children have no use.
+// (1) Sampled: blockIdx = (kRuns chunks, node, side).  The drafter's rows of nodes without
+// children have no use.
 template <int kRuns>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(TreeVerifyParams p) {
+  __shared__ double table[32];
   __shared__ float sm[kThreads / 64];
-  __shared__ double ss[kThreads / 64];
-  const int t = blockIdx.y, side = blockIdx.z, c = blockIdx.x;
+  __shared__ double ss[kRuns][kThreads / 64];
+  load_arguments(p);
+  const int t = blockIdx.y, side = blockIdx.z, c = blockIdx.x * kRuns, lane = threadIdx.x & 63;
   const uint16_t* row = side ? p.draft + t * p.ldd : p.target + t * p.ldt;
-  const int v0 = c * p.chunk + 8 * threadIdx.x;
+  const int v0 = c * kVerifyChunk + 8 * threadIdx.x;
   float x[kRuns][8];
 #pragma unroll
-  for (int r = 0; r < kRuns; ++r) load8(row, v0 + 8 * kThreads * r, p.vocab, x[r]);
+  for (int r = 0; r < kRuns; ++r) load8(row, v0 + kVerifyChunk * r, p.vocab, x[r]);
   if (side) {
     bool child = false;
     for (int s = t + 1 + threadIdx.x; s < p.nodes; s += kThreads) child |= p.parents[s] == t;
     if (!__syncthreads_or(child)) return;
   }
+  load_table(table);
   float m = -__builtin_inff();
 #pragma unroll
   for (int r = 0; r < kRuns; ++r)
 #pragma unroll
     for (int e = 0; e < 8; ++e) m = fmaxf(m, x[r][e]);            // fmaxf passes NaN over
   m = wave64_max(m);
-  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+  if (lane == 0) sm[threadIdx.x >> 6] = m;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kThreads / 64; ++w) m = fmaxf(m, sm[w]);
   const Scale sc = make_scale(m, p.scale_log2);
-  double s = 0.0;
 #pragma unroll
   for (int r = 0; r < kRuns; ++r) {
     double w[8];
-    weights8(x[r], v0 + 8 * kThreads * r, p.vocab, sc, w);
-    s += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+    weights8(x[r], v0 + kVerifyChunk * r, p.vocab, sc, table, w);
+    const double s = wave_sum(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
+    if (lane == 0) ss[r][threadIdx.x >> 6] = s;
   }
-  s = wave_sum(s);
-  if ((threadIdx.x & 63) == 0) ss[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < kThreads / 64; ++w) s += ss[w];
-    const long long at = ((long long)side * p.nodes + t) * p.chunks + c;
-    p.maxes[at] = m;
-    p.sums[at] = s;
+    const long long row_at = (long long)side * p.nodes + t;
+    double all = 0.0;
+#pragma unroll
+    for (int r = 0; r < kRuns; ++r) {
+      double s = ss[r][0];
+      for (int w = 1; w < kThreads / 64; ++w) s += ss[r][w];
+      if (c + r < p.chunks) p.sums[row_at * p.chunks + c + r] = s;
+      all += s;                                        // 0 past the row's end
+    }
+    p.maxes[row_at * p.groups + blockIdx.x] = m;
+    p.group_sums[row_at * p.groups + blockIdx.x] = all;
   }
 }
 
@@ -158,17 +195,18 @@ template <int kRuns>
 __global__ __launch_bounds__(kThreads) void verify_argmax_kernel(TreeVerifyParams p) {
   __shared__ float sm[kThreads / 64];
   __shared__ int si[kThreads / 64];
+  load_arguments(p);
   const int t = blockIdx.y, c = blockIdx.x;
   const uint16_t* row = p.target + t * p.ldt;
-  const int v0 = c * p.chunk + 8 * threadIdx.x;
+  const int v0 = c * kRuns * kVerifyChunk + 8 * threadIdx.x;
   float x[kRuns][8];
 #pragma unroll
-  for (int r = 0; r < kRuns; ++r) load8(row, v0 + 8 * kThreads * r, p.vocab, x[r]);
+  for (int r = 0; r < kRuns; ++r) load8(row, v0 + kVerifyChunk * r, p.vocab, x[r]);
   float m = -__builtin_inff();
   int at = 0x7fffffff;
 #pragma unroll
   for (int r = 0; r < kRuns; ++r) {
-    const int v = v0 + 8 * kThreads * r;
+    const int v = v0 + kVerifyChunk * r;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (v + e < p.vocab && x[r][e] == x[r][e]) better(m, at, x[r][e], v + e);
@@ -182,24 +220,56 @@ __global__ __launch_bounds__(kThreads) void verify_argmax_kernel(TreeVerifyParam
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < kThreads / 64; ++w) better(m, at, sm[w], si[w]);
-    p.maxes[(long long)t * p.chunks + c] = m;
-    p.args[(long long)t * p.chunks + c] = at;
+    p.maxes[(long long)t * p.groups + c] = m;
+    p.args[(long long)t * p.groups + c] = at;
   }
 }
 
 // A row's largest logit and its sum of weights relative to it, by one wave.
-__device__ __forceinline__ void row_stats(const TreeVerifyParams& p, int side, int t, int lane, float& m, double& z) {
-  const long long at = ((long long)side * p.nodes + t) * p.chunks;
-  const bool first = lane < p.chunks;                  // the lane's first chunk, loaded once
+__device__ __forceinline__ void row_stats(const TreeVerifyParams& p, const double* table, int side, int t, int lane, float& m,
+                                          double& z) {
+  const long long at = ((long long)side * p.nodes + t) * p.groups;
+  const bool first = lane < p.groups;                  // the lane's first group, loaded once
   const float m0 = first ? p.maxes[at + lane] : -__builtin_inff();
-  const double s0 = first ? p.sums[at + lane] : 0.0;
+  const double s0 = first ? p.group_sums[at + lane] : 0.0;
   m = m0;
-  for (int c = lane + 64; c < p.chunks; c += 64) m = fmaxf(m, p.maxes[at + c]);
+  for (int c = lane + 64; c < p.groups; c += 64) m = fmaxf(m, p.maxes[at + c]);
   m = wave64_max(m);
   const Scale sc = make_scale(m, p.scale_log2);
-  z = first ? s0 * weight(m0, sc) : 0.0;
-  for (int c = lane + 64; c < p.chunks; c += 64) z += p.sums[at + c] * weight(p.maxes[at + c], sc);
+  z = first ? s0 * weight(m0, sc, table) : 0.0;
+  for (int c = lane + 64; c < p.groups; c += 64) z += p.group_sums[at + c] * weight(p.maxes[at + c], sc, table);
   z = wave_sum(z);
+}
+
+// The same by 16 lanes (four rows per wave at once).
+__device__ __forceinline__ double row16_sum64(double x) {
+#pragma unroll
+  for (int d = 8; d; d >>= 1) x += __shfl_xor(x, d);
+  return x;
+}
+// (With weight_call: only the one-workgroup kernel uses it.)
+__device__ __forceinline__ void row_stats16(const TreeVerifyParams& p, const double* table, int side, int t, int c, float& m,
+                                            double& z) {
+  const long long at = ((long long)side * p.nodes + t) * p.groups;
+  float mc[2];                                         // the lane's first two groups, loaded once
+  double sc[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const bool in = c + 16 * i < p.groups;
+    mc[i] = in ? p.maxes[at + c + 16 * i] : -__builtin_inff();
+    sc[i] = in ? p.group_sums[at + c + 16 * i] : 0.0;
+  }
+  m = fmaxf(mc[0], mc[1]);
+  for (int i = c + 32; i < p.groups; i += 16) m = fmaxf(m, p.maxes[at + i]);
+  m = row16_max(m);
+  z = 0.0;
+#pragma unroll 1
+  for (int i = c; i < p.groups; i += 16) {
+    const float mi = i == c ? mc[0] : i == c + 16 ? mc[1] : p.maxes[at + i];
+    const double si = i == c ? sc[0] : i == c + 16 ? sc[1] : p.group_sums[at + i];
+    z += si * weight_call(mi, m, p.scale_log2, table);
+  }
+  z = row16_sum64(z);
 }
 
 // The sum over chunks of round r (from 1) of node t, by one wave.
@@ -227,8 +297,9 @@ __device__ __forceinline__ float logit(const uint16_t* row, int v) {
   return (float)reinterpret_cast<const _Float16*>(row)[v];
 }
 // Probability of token x in a row; 0 outside the vocabulary.
-__device__ __forceinline__ double probability(const uint16_t* row, int x, int vocab, const Scale& s, double z) {
-  return x >= 0 && x < vocab ? weight(logit(row, x), s) / z : 0.0;
+__device__ __forceinline__ double probability(const uint16_t* row, int x, int vocab, const Scale& s, double z,
+                                              const double* table) {
+  return x >= 0 && x < vocab ? weight(logit(row, x), s, table) / z : 0.0;
 }
 
 // (2) Round `round` of drawn drafts: blockIdx = (chunk, node).  Each wave finds out for itself
@@ -236,8 +307,10 @@ __device__ __forceinline__ double probability(const uint16_t* row, int x, int vo
 // meanwhile.
 template <int kRuns>
 __global__ __launch_bounds__(kThreads) void verify_round_kernel(TreeVerifyParams p, int round) {
-  __shared__ double ss[kThreads / 64];
-  const int t = blockIdx.y, c = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ double table[32];
+  __shared__ double ss[kRuns][kThreads / 64];
+  load_arguments(p);
+  const int t = blockIdx.y, c = blockIdx.x * kRuns, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint16_t* rp = p.target + t * p.ldt;
   const uint16_t* rq = p.draft + t * p.ldd;
   int child = -1, found = 0;                           // lane k: the node's child k (from 0), k < round
@@ -248,23 +321,25 @@ __global__ __launch_bounds__(kThreads) void verify_round_kernel(TreeVerifyParams
       if (lane == found) child = s0 + __builtin_ctzll(hits);
   }
   if (found < round) return;                           // the same in every wave
-  const int v0 = c * p.chunk + 8 * threadIdx.x;
+  load_table(table);
+  const int v0 = c * kVerifyChunk + 8 * threadIdx.x;
   float x[kRuns][8], y[kRuns][8];
 #pragma unroll
   for (int i = 0; i < kRuns; ++i) {
-    load8(rp, v0 + 8 * kThreads * i, p.vocab, x[i]);
-    load8(rq, v0 + 8 * kThreads * i, p.vocab, y[i]);
+    load8(rp, v0 + kVerifyChunk * i, p.vocab, x[i]);
+    load8(rq, v0 + kVerifyChunk * i, p.vocab, y[i]);
   }
+  __syncthreads();
   float mp, mq;
   double zp, zq;
-  row_stats(p, 0, t, lane, mp, zp);
-  row_stats(p, 1, t, lane, mq, zq);
+  row_stats(p, table, 0, t, lane, mp, zp);
+  row_stats(p, table, 1, t, lane, mq, zq);
   const Scale sp = make_scale(mp, p.scale_log2), sq = make_scale(mq, p.scale_log2);
   double pw = 0.0, uq = 0.0, qw = 0.0;
   if (child >= 0) {
     const int tok = p.tokens[child];
-    pw = probability(rp, tok, p.vocab, sp, zp);
-    qw = probability(rq, tok, p.vocab, sq, zq);
+    pw = probability(rp, tok, p.vocab, sp, zp, table);
+    qw = probability(rq, tok, p.vocab, sq, zq, table);
     uq = (double)p.accept_u[child] * qw;
   }
   Residual r{0.0, 1.0, 0};
@@ -273,41 +348,45 @@ __global__ __launch_bounds__(kThreads) void verify_round_kernel(TreeVerifyParams
     if (ok) return;                                    // a child stands: no later round is looked at
     if (k + 1 < round) reject(p, t, k + 1, lane, r);
   }
-  double s = 0.0;
-  if (r.round == round - 1) {                          // else an earlier round's sum was 0
-    const double a = (r.a + r.s) / zq, ip = 1.0 / zp;
+  const double a = (r.a + r.s) / zq, ip = 1.0 / zp;
 #pragma unroll
-    for (int i = 0; i < kRuns; ++i) {
-      const int v = v0 + 8 * kThreads * i;
+  for (int i = 0; i < kRuns; ++i) {
+    double s = 0.0;
+    if (r.round == round - 1) {                        // else an earlier round's sum was 0
+      const int v = v0 + kVerifyChunk * i;
       double wp[8], wq[8];
-      weights8(x[i], v, p.vocab, sp, wp);
-      weights8(y[i], v, p.vocab, sq, wq);
+      weights8(x[i], v, p.vocab, sp, table, wp);
+      weights8(y[i], v, p.vocab, sq, table, wq);
 #pragma unroll
       for (int e = 0; e < 8; ++e) s += fmax(wp[e] * ip - wq[e] * a, 0.0);
     }
+    s = wave_sum(s);
+    if (lane == 0) ss[i][wave] = s;
   }
-  s = wave_sum(s);
-  if (lane == 0) ss[wave] = s;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kThreads / 64; ++w) s += ss[w];
-    p.rounds[((long long)(round - 1) * p.nodes + t) * p.chunks + c] = s;
+  if (threadIdx.x < kRuns && c + (int)threadIdx.x < p.chunks) {
+    double s = ss[threadIdx.x][0];
+    for (int w = 1; w < kThreads / 64; ++w) s += ss[threadIdx.x][w];
+    p.rounds[((long long)(round - 1) * p.nodes + t) * p.chunks + c + threadIdx.x] = s;
   }
 }
 
 // (3) One workgroup.
 constexpr int kWalkThreads = 1024;
 constexpr int kWalkWaves = kWalkThreads / 64;
-constexpr int kMaxChunk = 8 * kWalkThreads;            // the last token's chunk: 8 logits per thread
+constexpr int kMaxChunks = (1 << 24) / kVerifyChunk;   // of the largest vocabulary
 
 struct WalkShared {
+  double table[32];
   int parent[kNodes], token[kNodes], next[kNodes], path[kNodes], best[kNodes];
   float mp[kNodes], mq[kNodes], u[kNodes];
   double zp[kNodes], zq[kNodes];
   double pw[kNodes], qw[kNodes];                       // a node's token in its parent's distributions
   double wave[kWalkWaves];
-  unsigned gone[kMaxChunk / 32];                       // rejected tokens of one chunk
-  int count, chunk, first, tail;
+  unsigned gone[kVerifyChunk / 32];                       // rejected tokens of one chunk
+  double sums[kMaxChunks];                             // of the last token's row
+  int hit[kWalkWaves], tail[kWalkWaves];
+  int count, chunk;
   double before, total;
 };
 
@@ -325,9 +404,11 @@ __device__ __forceinline__ double block_sum(double x, WalkShared& sh) {
 
 __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyParams p) {
   __shared__ WalkShared sh;
+  load_arguments(p);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const bool drawn = !p.greedy && p.draft != nullptr;
   const float sample_u = p.greedy ? 0.0f : *p.sample_u;
+  if (!p.greedy) load_table(sh.table);
   for (int t = tid; t < p.nodes; t += kWalkThreads) {
     const int parent = t ? p.parents[t] : -1;
     sh.parent[t] = parent < t ? parent : -1;           // otherwise never reached
@@ -335,29 +416,27 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
     sh.u[t] = t && !p.greedy ? p.accept_u[t] : 0.0f;
     sh.next[t] = -1;
   }
-  for (int t = wave; t < p.nodes; t += kWalkWaves) {
+  __syncthreads();
+  for (int t0 = 4 * wave; t0 < p.nodes; t0 += 4 * kWalkWaves) {   // four rows per wave, 16 lanes each
+    const int c0 = lane & 15, t = min(t0 + (lane >> 4), p.nodes - 1);
     if (p.greedy) {
       float m = -__builtin_inff();
       int at = 0x7fffffff;
-      for (int c = lane; c < p.chunks; c += 64)
-        better(m, at, p.maxes[(long long)t * p.chunks + c], p.args[(long long)t * p.chunks + c]);
+      for (int c = c0; c < p.groups; c += 16)
+        better(m, at, p.maxes[(long long)t * p.groups + c], p.args[(long long)t * p.groups + c]);
 #pragma unroll
-      for (int d = 32; d; d >>= 1) better(m, at, __shfl_xor(m, d), __shfl_xor(at, d));
-      if (lane == 0) sh.best[t] = at == 0x7fffffff ? 0 : at;
+      for (int d = 8; d; d >>= 1) better(m, at, __shfl_xor(m, d), __shfl_xor(at, d));
+      if (c0 == 0) sh.best[t] = at == 0x7fffffff ? 0 : at;
     } else {
-      float m;
-      double z;
-      row_stats(p, 0, t, lane, m, z);
-      if (lane == 0) {
+      float m, mq = 0.0f;
+      double z, zq = 1.0;
+      row_stats16(p, sh.table, 0, t, c0, m, z);
+      if (drawn) row_stats16(p, sh.table, 1, t, c0, mq, zq);     // of a node without children: not written, not used
+      if (c0 == 0) {
         sh.mp[t] = m;
         sh.zp[t] = z;
-      }
-      if (drawn) {                                     // of a node without children: not written, not used
-        row_stats(p, 1, t, lane, m, z);
-        if (lane == 0) {
-          sh.mq[t] = m;
-          sh.zq[t] = z;
-        }
+        sh.mq[t] = mq;
+        sh.zq[t] = zq;
       }
     }
   }
@@ -367,10 +446,11 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
       const int t = sh.parent[s], x = sh.token[s];
       double pw = 0.0, qw = 0.0;
       if (t >= 0) {
-        pw = probability(p.target + t * p.ldt, x, p.vocab, make_scale(sh.mp[t], p.scale_log2), sh.zp[t]);
-        if (drawn)
-          qw = probability(p.draft + t * p.ldd, x, p.vocab, make_scale(sh.mq[t], p.scale_log2), sh.zq[t]);
-        else                                           // a sibling's token that was rejected has nothing left
+        const bool in = x >= 0 && x < p.vocab;
+        const float lp = in ? logit(p.target + t * p.ldt, x) : 0.0f, lq = in && drawn ? logit(p.draft + t * p.ldd, x) : 0.0f;
+        if (in) pw = weight_call(lp, sh.mp[t], p.scale_log2, sh.table) / sh.zp[t];
+        if (in && drawn) qw = weight_call(lq, sh.mq[t], p.scale_log2, sh.table) / sh.zq[t];
+        if (!drawn)                                           // a sibling's token that was rejected has nothing left
           for (int b = t + 1; b < s; ++b)
             if (sh.parent[b] == t && sh.token[b] == x) pw = 0.0;
       }
@@ -412,8 +492,6 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
     int n = 0, t = 0;
     for (; t >= 0; t = sh.next[t]) sh.path[n++] = t;
     sh.count = n;
-    sh.first = 0x7fffffff;
-    sh.tail = -1;
     sh.chunk = -1;
   }
   __syncthreads();
@@ -426,7 +504,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
     // The last token: choose a chunk by the chunks' sums of what is left of the distribution,
     // then the index in it.
     const uint16_t* rp = p.target + node * p.ldt;
-    const Scale sp = make_scale(sh.mp[node], p.scale_log2);
+    const float mp = sh.mp[node];
     const double ip = 1.0 / sh.zp[node];
     Residual r{0.0, 1.0, 0};
     int children = 0;
@@ -436,7 +514,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
       for (int k = 1; k <= min(children, p.max_children); ++k) reject(p, node, k, lane, r);
     const double a = r.round ? r.a / sh.zq[node] : 0.0;
     const uint16_t* rq = r.round ? p.draft + node * p.ldd : nullptr;
-    const Scale sq = make_scale(r.round ? sh.mq[node] : 0.0f, p.scale_log2);
+    const float mq = r.round ? sh.mq[node] : 0.0f;
     const double* rs = r.round ? p.rounds + ((long long)(r.round - 1) * p.nodes + node) * p.chunks : nullptr;
     const bool holes = !drawn && children;             // rejected tokens of point drafts
 
@@ -444,30 +522,26 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
     auto chunk_weights = [&](int c, double (&w)[8]) {
       if (holes) {
         __syncthreads();                               // sh.gone may still be read
-        for (int i = tid; i < kMaxChunk / 32; i += kWalkThreads) sh.gone[i] = 0u;
+        if (tid < kVerifyChunk / 32) sh.gone[tid] = 0u;
         __syncthreads();
         for (int s = node + 1 + tid; s < p.nodes; s += kWalkThreads) {
-          const int x = sh.token[s] - c * p.chunk;
-          if (sh.parent[s] == node && sh.token[s] >= 0 && x >= 0 && x < p.chunk) atomicOr(&sh.gone[x >> 5], 1u << (x & 31));
+          const int x = sh.token[s] - c * kVerifyChunk;
+          if (sh.parent[s] == node && sh.token[s] >= 0 && x >= 0 && x < kVerifyChunk) atomicOr(&sh.gone[x >> 5], 1u << (x & 31));
         }
         __syncthreads();
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e] = 0.0;
-      const int i0 = 8 * tid, v = c * p.chunk + i0;
-      if (i0 >= p.chunk || v >= p.vocab) return;
-      float x[8];
+      const int i0 = 8 * tid, v = c * kVerifyChunk + i0;
+      if (i0 >= kVerifyChunk || v >= p.vocab) return;
+      float x[8], y[8];
       load8(rp, v, p.vocab, x);
-      weights8(x, v, p.vocab, sp, w);
+      if (rq) load8(rq, v, p.vocab, y);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] *= ip;
+      for (int e = 0; e < 8; ++e) w[e] = v + e < p.vocab ? weight_call(x[e], mp, p.scale_log2, sh.table) * ip : 0.0;
       if (rq) {
-        float y[8];
-        double wq[8];
-        load8(rq, v, p.vocab, y);
-        weights8(y, v, p.vocab, sq, wq);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = fmax(w[e] - wq[e] * a, 0.0);
+        for (int e = 0; e < 8; ++e) w[e] = fmax(w[e] - weight_call(y[e], mq, p.scale_log2, sh.table) * a, 0.0);
       }
       if (holes) {
         const unsigned gone = (sh.gone[i0 >> 5] >> (i0 & 31)) & 0xffu;
@@ -476,16 +550,16 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
       }
     };
 
-    // Chunk sums into global scratch (the node's own: nothing else reads it any more).  Point
-    // drafts: without the rejected tokens' weights, subtracted where enough is left that the
-    // rounding of the subtraction does not matter, else summed again.
-    double* sums = p.sums + (long long)node * p.chunks;
+    // Chunk sums.  Point drafts: without the rejected tokens' weights, subtracted where enough is
+    // left that the rounding of the subtraction does not matter, else summed again.
+    double* sums = sh.sums;
     for (int c = tid; c < p.chunks; c += kWalkThreads) {
-      double s = rs ? rs[c] : sums[c] * weight(p.maxes[(long long)node * p.chunks + c], sp) * ip;
+      const long long at = (long long)node * p.chunks + c;
+      double s = rs ? rs[c] : p.sums[at] * weight_call(p.maxes[(long long)node * p.groups + c / p.runs], mp, p.scale_log2, sh.table) * ip;
       if (holes) {
         const double all = s;
         for (int k = node + 1; k < p.nodes; ++k)
-          if (sh.parent[k] == node && sh.token[k] >= 0 && sh.token[k] / p.chunk == c) s -= sh.pw[k];
+          if (sh.parent[k] == node && sh.token[k] >= 0 && sh.token[k] / kVerifyChunk == c) s -= sh.pw[k];
         if (s < 1e-3 * all) s = -1.0;                  // to be summed again
       }
       sums[c] = s;
@@ -494,7 +568,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
     if (holes)
       for (int k = node + 1; k < p.nodes; ++k) {       // only these chunks can be marked
         if (sh.parent[k] != node || sh.token[k] < 0 || sh.token[k] >= p.vocab) continue;
-        const int c = sh.token[k] / p.chunk;
+        const int c = sh.token[k] / kVerifyChunk;
         if (sums[c] >= 0.0) continue;                  // uniform: nothing is written between the barriers
         double w[8];
         chunk_weights(c, w);
@@ -552,21 +626,34 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
       __syncthreads();                                 // sh.wave may still be read
       if (lane == 63) sh.wave[wave] = end;
       __syncthreads();
-      double cum = sh.before + (end - run);
-      for (int i = 0; i < wave; ++i) cum += sh.wave[i];
-      int hit = 0x7fffffff, tail = -1;
+      double ahead = lane < wave ? sh.wave[lane] : 0.0;  // the waves before this one
+#pragma unroll
+      for (int d = 8; d; d >>= 1) ahead += __shfl_xor(ahead, d);
+      double cum = sh.before + __shfl(ahead, 0) + (end - run);
+      int hit = -1, tail = -1;                         // the thread's first past the goal, and last with weight
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         cum += w[e];
         if (w[e] > 0.0) {
           tail = 8 * tid + e;
-          if (cum > goal && hit == 0x7fffffff) hit = 8 * tid + e;
+          if (cum > goal && hit < 0) hit = 8 * tid + e;
         }
       }
-      if (hit != 0x7fffffff) atomicMin(&sh.first, hit);
-      if (tail >= 0) atomicMax(&sh.tail, tail);
+      // The first hit in index order, else the last tail.  (Not by LDS atomics: over a wave's
+      // lanes those run one lane at a time.)
+      const unsigned long long hits = __ballot(hit >= 0), tails = __ballot(tail >= 0);
+      const int h = __shfl(hit, hits ? __builtin_ctzll(hits) : 0), tl = __shfl(tail, tails ? 63 - __builtin_clzll(tails) : 0);
+      if (lane == 0) {
+        sh.hit[wave] = hits ? h : -1;
+        sh.tail[wave] = tails ? tl : -1;
+      }
       __syncthreads();
-      last = chunk * p.chunk + (sh.first != 0x7fffffff ? sh.first : max(sh.tail, 0));
+      int first = -1, final = 0;
+#pragma unroll
+      for (int i = kWalkWaves - 1; i >= 0; --i) first = sh.hit[i] >= 0 ? sh.hit[i] : first;
+#pragma unroll
+      for (int i = 0; i < kWalkWaves; ++i) final = sh.tail[i] >= 0 ? sh.tail[i] : final;
+      last = chunk * kVerifyChunk + (first >= 0 ? first : final);
     }
   }
 
@@ -580,19 +667,19 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
 template <int kRuns>
 void launch_passes(const TreeVerifyParams& p, hipStream_t stream) {
   if (p.greedy) {
-    hipLaunchKernelGGL(verify_argmax_kernel<kRuns>, dim3(p.chunks, p.nodes), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL(verify_argmax_kernel<kRuns>, dim3(p.groups, p.nodes), dim3(kThreads), 0, stream, p);
     return;
   }
-  hipLaunchKernelGGL(verify_stats_kernel<kRuns>, dim3(p.chunks, p.nodes, p.draft ? 2 : 1), dim3(kThreads), 0, stream, p);
+  hipLaunchKernelGGL(verify_stats_kernel<kRuns>, dim3(p.groups, p.nodes, p.draft ? 2 : 1), dim3(kThreads), 0, stream, p);
   if (p.draft)
     for (int r = 1; r <= p.max_children; ++r)
-      hipLaunchKernelGGL(verify_round_kernel<kRuns>, dim3(p.chunks, p.nodes), dim3(kThreads), 0, stream, p, r);
+      hipLaunchKernelGGL(verify_round_kernel<kRuns>, dim3(p.groups, p.nodes), dim3(kThreads), 0, stream, p, r);
 }
 
 }  // namespace
 
 hipError_t launch_tree_verify(const TreeVerifyParams& p, hipStream_t stream) {
-  if (p.chunk == 8 * kThreads * 4)
+  if (p.runs == 4)
     launch_passes<4>(p, stream);
   else
     launch_passes<1>(p, stream);

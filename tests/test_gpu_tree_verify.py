@@ -280,3 +280,10 @@ def test_two_streams_at_once(qdiy):
     torch.cuda.synchronize()
     for c in cs:
         assert c.got() == c.want()
+
+
+@pytest.mark.parametrize("mode", MODES)
+def test_a_vocabulary_of_many_chunks(qdiy, mode):
+    """More chunks than a wave's lanes, in the short and in the long chunks."""
+    Case(2, 300001, mode, seed=2, parents=[-1, 0]).check(qdiy)
+    Case(3, 4500000, mode, seed=3, parents=[-1, 0, 0]).check(qdiy)
