@@ -95,11 +95,15 @@ inline TreeAttnPlan tree_attn_plan(int nodes, int heads, int kv_heads, int prefi
 }
 hipError_t launch_tree_attention(const TreeAttnParams& p, const TreeAttnPlan& plan, hipStream_t stream);
 
-// Logits of a row per chunk of the verification's passes, and chunks per workgroup: 4, or 1 where
-// that would be fewer than two workgroups per CU (5 rows of 151936 logits: the argmax pass 3.8
-// us against 5.8).
+// Logits of a row per chunk of the verification's passes, and chunks per workgroup: as many as
+// leave two workgroups per CU (more would be dispatched one after the other, fewer leave CUs
+// empty: 5 rows of 151936 logits, argmax pass, 3.8 us at 1 chunk, 5.8 at 4), at most 16.
 constexpr int kVerifyChunk = 2048;
-inline int verify_runs(int nodes, int chunks) { return (long long)nodes * ((chunks + 3) / 4) >= 512 ? 4 : 1; }
+constexpr int kVerifyRuns = 16;
+inline int verify_runs(int nodes, int chunks) {
+  const long long n = (long long)nodes * chunks / 1024;
+  return n < 1 ? 1 : n > kVerifyRuns ? kVerifyRuns : (int)n;
+}
 
 struct TreeVerifyParams {
   const uint16_t* target;   // [nodes][vocab]

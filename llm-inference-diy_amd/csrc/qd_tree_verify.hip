@@ -41,61 +41,61 @@ __device__ __forceinline__ void load_arguments(const TreeVerifyParams& p) {
 }
 
 // Weight of a logit in a row (or chunk): `m` its largest logit, `scale` 32 log2(e) / temperature
-// (exponents are counted in 32nds).
+// (exponents are counted in 32nds), `least` the smallest logit that still has one.
 struct Scale {
-  float m;
+  float m, least;
   double md, scale;
 };
-__device__ __forceinline__ Scale make_scale(float m, double scale) { return Scale{m, (double)m, scale}; }
-
-// 2^(j / 32).
-__device__ const double kPow32[32] = {
-    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
-    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
-    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
-    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
-    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
-    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
-    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
-    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0,
-};
-// Each workgroup's copy, 256 bytes: one entry per pair of LDS banks, so lanes never conflict.
-__device__ __forceinline__ void load_table(double* table) {
-  if (threadIdx.x < 32) table[threadIdx.x] = kPow32[threadIdx.x];
+constexpr double kLeast = 28800.0;                     // 2^-900
+__device__ __forceinline__ Scale make_scale(float m, double scale) {
+  return Scale{m, m - (float)(kLeast / scale), (double)m, scale};
 }
+// What a sum may hold of weights that should be 0 (2^24 of 2^-900) counts as 0.
+constexpr double kNothing = 1e-250;
 
-// 2^(x / 32), x = (l - m) * scale <= 0, to a relative 2e-12: 2^n 2^(j/32) times the series of
-// 2^(f/32) to degree 4 on |f| <= 1/2 (remainder (ln2/64)^5 / 5! = 1.3e-12; the difference of two
-// halves is exact).  Rounding to 32 n + j by adding 1.5 * 2^52 leaves it in the low word, and
-// adding n to the exponent field scales: the stats pass is bound by fp64 instructions, of
-// which this takes 11 (a series on |f| <= 1/2 of a whole exponent takes 18, and the pass over 64
-// rows of 151936 logits 13.0 us instead of KSTATS).  Below 2^-1000: 0, as for NaN (fmaxf drops
-// it).  m is finite.
-__device__ __forceinline__ double weight_finite(float l, const Scale& s, const double* table) {
-  const double x = ((double)l - s.md) * s.scale;
+// 2^(j / 32) for j < 32, with j << 15 taken off the high word: adding n << 15 to it gives
+// 2^(n / 32) for n = 32 q + j.
+__device__ const unsigned long long kPow32[32] = {
+    0x3ff0000000000000, 0x3fefd9b0d3158574, 0x3fefb5586cf9890f, 0x3fef9301d0125b51,
+    0x3fef72b83c7d517b, 0x3fef54873168b9aa, 0x3fef387a6e756238, 0x3fef1e9df51fdee1,
+    0x3fef06fe0a31b715, 0x3feef1a7373aa9cb, 0x3feedea64c123422, 0x3feece086061892d,
+    0x3feebfdad5362a27, 0x3feeb42b569d4f82, 0x3feeab07dd485429, 0x3feea47eb03a5585,
+    0x3feea09e667f3bcd, 0x3fee9f75e8ec5f74, 0x3feea11473eb0187, 0x3feea589994cce13,
+    0x3feeace5422aa0db, 0x3feeb737b0cdc5e5, 0x3feec49182a3f090, 0x3feed503b23e255d,
+    0x3feee89f995ad3ad, 0x3feeff76f2fb5e47, 0x3fef199bdd85529c, 0x3fef3720dcef9069,
+    0x3fef5818dcfba487, 0x3fef7c97337b9b5f, 0x3fefa4afa2a490da, 0x3fefd0765b6e4540,
+};
+
+// 2^(x / 32), x = (l - m) * scale <= 0, to a relative 2e-12: 2^(n/32) times the series of 2^(f/32)
+// to degree 4 on |f| <= 1/2 (remainder (ln2/64)^5 / 5! = 1.3e-12; the difference of two halves is
+// exact).  Rounding to n by adding 1.5 * 2^52 leaves it in the low word.  A NaN, and whatever
+// weighs less than 2^-900, counts as 2^-900.  m is finite.  The passes are bound by the number
+// of instructions, of which this takes 16 (fp64 ones issue at the fp32 rate): KSTATS.
+// table: the workgroup's copy of kPow32 in LDS, 256 bytes: one entry per pair of banks, so
+// lanes never conflict.
+__device__ __forceinline__ double weight_finite(float l, const Scale& s, const unsigned long long* table) {
+  const double x = ((double)fmaxf(l, s.least) - s.md) * s.scale;
   const double t = x + 0x1.8p52;
   const double f = x - (t - 0x1.8p52);
-  const int n = (int)__builtin_bit_cast(long long, t);
+  const unsigned n = (unsigned)__builtin_bit_cast(unsigned long long, t);
+  const unsigned long long bits = table[n & 31];
+  const double base = __builtin_bit_cast(double, ((unsigned long long)((unsigned)(bits >> 32) + (n << 15)) << 32) | (unsigned)bits);
   double r = 9.172562701824643e-09;                    // (ln2 / 32)^k / k!, k = 4 .. 1
   r = __builtin_fma(r, f, 1.6938509724371819e-06);
   r = __builtin_fma(r, f, 0.00023459619820224677);
   r = __builtin_fma(r, f, 0.02166084939249829);
-  const double base = table[n & 31];
-  const long long bits = __builtin_bit_cast(long long, __builtin_fma(base, r * f, base));
-  const int lo = (int)bits, hi = (int)(bits >> 32) + ((n >> 5) << 20);
-  const double w = __builtin_bit_cast(double, ((long long)hi << 32) | (unsigned)lo);
-  return x > -32000.0 ? w : 0.0;                       // and where x is NaN
+  return __builtin_fma(base, r * f, base);
 }
-// The same for any m: the largest logits weigh 1 also where they are infinite.
-__device__ __forceinline__ double weight(float l, const Scale& s, const double* table) {
-  if (fabsf(s.m) < __builtin_inff()) return weight_finite(l, s, table);
+// The same for any m, and 0 where there is no weight: the largest logits weigh 1 also where they
+// are infinite.
+__device__ __forceinline__ double weight(float l, const Scale& s, const unsigned long long* table) {
+  if (fabsf(s.m) < __builtin_inff()) return l > s.least ? weight_finite(l, s, table) : 0.0;
   if (l != l) l = -__builtin_inff();
   return l == s.m ? 1.0 : 0.0;
 }
-
 // The same as a function of its own, for the one-workgroup kernel: its time is that of fetching
 // instructions that run once, and an inlined weight is 40 of them.
-__device__ __attribute__((noinline)) double weight_call(float l, float m, double scale, const double* table) {
+__device__ __attribute__((noinline)) double weight_call(float l, float m, double scale, const unsigned long long* table) {
   return weight(l, make_scale(m, scale), table);
 }
 
@@ -105,20 +105,28 @@ __device__ __forceinline__ double wave_sum(double x) {
   return x;
 }
 
-// Eight logits from index v on; -inf past the row's end.
-__device__ __forceinline__ void load8(const uint16_t* row, int v, int vocab, float (&x)[8]) {
-  if (v + 8 <= vocab) {
-    const f16x8u a = *reinterpret_cast<const f16x8u*>(row + v);
+// Eight logits from index v on; -inf past the row's end.  In two steps, so that several runs'
+// loads are in flight together: fetch8 has no branch (it moves a run that passes the end back
+// into the row), expand8 reads such a run again, one by one.
+__device__ __forceinline__ f16x8u fetch8(const uint16_t* row, int v, int vocab) {
+  if (vocab < 8) return f16x8u{};                      // uniform: expand8 reads them all
+  return *reinterpret_cast<const f16x8u*>(row + min(v, vocab - 8));
+}
+__device__ __forceinline__ void expand8(const f16x8u& raw, const uint16_t* row, int v, int vocab, float (&x)[8]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = (float)a[e];
-  } else {
+  for (int e = 0; e < 8; ++e) x[e] = (float)raw[e];
+  if (v + 8 > vocab) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       x[e] = v + e < vocab ? (float)reinterpret_cast<const _Float16*>(row)[v + e] : -__builtin_inff();
   }
 }
+__device__ __forceinline__ void load8(const uint16_t* row, int v, int vocab, float (&x)[8]) {
+  expand8(fetch8(row, v, vocab), row, v, vocab, x);
+}
+
 // Their weights; 0 past the row's end.
-__device__ __forceinline__ void weights8(const float (&x)[8], int v, int vocab, const Scale& s, const double* table,
+__device__ __forceinline__ void weights8(const float (&x)[8], int v, int vocab, const Scale& s, const unsigned long long* table,
                                          double (&w)[8]) {
   if (fabsf(s.m) < __builtin_inff()) {                 // uniform over a chunk
 #pragma unroll
@@ -129,57 +137,59 @@ __device__ __forceinline__ void weights8(const float (&x)[8], int v, int vocab, 
   }
 }
 
-// (1) Sampled: blockIdx = (kRuns chunks, node, side).  The drafter's rows of nodes without
-// children have no use.
-template <int kRuns>
+// (1) Sampled: blockIdx = (p.runs chunks, node, side).  The drafter's rows of nodes without
+// children have no use.  Each wave sums each run of 512 logits relative to the run's own
+// largest, so that its work on one run stands behind that run's load alone; one wave puts the
+// sums on a common base at the end.
+constexpr int kWaves = kThreads / 64;
+static_assert(kVerifyRuns * kWaves <= 64, "a workgroup's parts are one wave's lanes");
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(TreeVerifyParams p) {
-  __shared__ double table[32];
-  __shared__ float sm[kThreads / 64];
-  __shared__ double ss[kRuns][kThreads / 64];
+  __shared__ unsigned long long table[32];
+  __shared__ float sm[64];                             // [run][wave]
+  __shared__ double ss[64];
   load_arguments(p);
-  const int t = blockIdx.y, side = blockIdx.z, c = blockIdx.x * kRuns, lane = threadIdx.x & 63;
+  const int t = blockIdx.y, side = blockIdx.z, c = blockIdx.x * p.runs, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint16_t* row = side ? p.draft + t * p.ldd : p.target + t * p.ldt;
   const int v0 = c * kVerifyChunk + 8 * threadIdx.x;
-  float x[kRuns][8];
-#pragma unroll
-  for (int r = 0; r < kRuns; ++r) load8(row, v0 + kVerifyChunk * r, p.vocab, x[r]);
+  f16x8u raw = fetch8(row, v0, p.vocab);
   if (side) {
     bool child = false;
     for (int s = t + 1 + threadIdx.x; s < p.nodes; s += kThreads) child |= p.parents[s] == t;
     if (!__syncthreads_or(child)) return;
   }
-  load_table(table);
-  float m = -__builtin_inff();
-#pragma unroll
-  for (int r = 0; r < kRuns; ++r)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m = fmaxf(m, x[r][e]);            // fmaxf passes NaN over
-  m = wave64_max(m);
-  if (lane == 0) sm[threadIdx.x >> 6] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) m = fmaxf(m, sm[w]);
-  const Scale sc = make_scale(m, p.scale_log2);
-#pragma unroll
-  for (int r = 0; r < kRuns; ++r) {
+  if (lane < 32) table[lane] = kPow32[lane];           // every wave writes it all, and needs no barrier to read it
+#pragma unroll 1
+  for (int r = 0; r < p.runs; ++r) {
+    const int v = v0 + kVerifyChunk * r;
+    float x[8], m = -__builtin_inff();
     double w[8];
-    weights8(x[r], v0 + kVerifyChunk * r, p.vocab, sc, table, w);
+    const f16x8u cur = raw;
+    raw = fetch8(row, v + kVerifyChunk, p.vocab);
+    expand8(cur, row, v, p.vocab, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, x[e]);    // fmaxf passes NaN over
+    m = wave64_max(m);
+    weights8(x, v, p.vocab, make_scale(m, p.scale_log2), table, w);
     const double s = wave_sum(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
-    if (lane == 0) ss[r][threadIdx.x >> 6] = s;
+    if (lane == 0) {
+      sm[r * kWaves + wave] = m;
+      ss[r * kWaves + wave] = s;
+    }
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    const long long row_at = (long long)side * p.nodes + t;
-    double all = 0.0;
+  if (wave == 0) {
+    const int parts = p.runs * kWaves;
+    const float m = lane < parts ? sm[lane] : -__builtin_inff(), mg = wave64_max(m);
+    double s = lane < parts ? ss[lane] * weight(m, make_scale(mg, p.scale_log2), table) : 0.0;
 #pragma unroll
-    for (int r = 0; r < kRuns; ++r) {
-      double s = ss[r][0];
-      for (int w = 1; w < kThreads / 64; ++w) s += ss[r][w];
-      if (c + r < p.chunks) p.sums[row_at * p.chunks + c + r] = s;
-      all += s;                                        // 0 past the row's end
+    for (int d = 1; d < kWaves; d <<= 1) s += __shfl_xor(s, d);   // the run's, in each of its lanes
+    const double all = wave_sum(lane % kWaves == 0 ? s : 0.0);    // 0 past the row's end
+    const long long row_at = (long long)side * p.nodes + t;
+    if (lane % kWaves == 0 && lane < parts && c + lane / kWaves < p.chunks) p.sums[row_at * p.chunks + c + lane / kWaves] = s;
+    if (lane == 0) {
+      p.maxes[row_at * p.groups + blockIdx.x] = mg;
+      p.group_sums[row_at * p.groups + blockIdx.x] = all;
     }
-    p.maxes[row_at * p.groups + blockIdx.x] = m;
-    p.group_sums[row_at * p.groups + blockIdx.x] = all;
   }
 }
 
@@ -191,25 +201,26 @@ __device__ __forceinline__ void better(float& m, int& i, float m2, int i2) {
     i = i2;
   }
 }
-template <int kRuns>
 __global__ __launch_bounds__(kThreads) void verify_argmax_kernel(TreeVerifyParams p) {
   __shared__ float sm[kThreads / 64];
   __shared__ int si[kThreads / 64];
   load_arguments(p);
   const int t = blockIdx.y, c = blockIdx.x;
   const uint16_t* row = p.target + t * p.ldt;
-  const int v0 = c * kRuns * kVerifyChunk + 8 * threadIdx.x;
-  float x[kRuns][8];
-#pragma unroll
-  for (int r = 0; r < kRuns; ++r) load8(row, v0 + kVerifyChunk * r, p.vocab, x[r]);
+  const int v0 = c * p.runs * kVerifyChunk + 8 * threadIdx.x;
+  f16x8u raw = fetch8(row, v0, p.vocab);
   float m = -__builtin_inff();
   int at = 0x7fffffff;
-#pragma unroll
-  for (int r = 0; r < kRuns; ++r) {
+#pragma unroll 1
+  for (int r = 0; r < p.runs; ++r) {
     const int v = v0 + kVerifyChunk * r;
+    const f16x8u cur = raw;
+    raw = fetch8(row, v + kVerifyChunk, p.vocab);
+    float x[8];
+    expand8(cur, row, v, p.vocab, x);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (v + e < p.vocab && x[r][e] == x[r][e]) better(m, at, x[r][e], v + e);
+      if (v + e < p.vocab && x[e] == x[e]) better(m, at, x[e], v + e);
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) better(m, at, __shfl_xor(m, d), __shfl_xor(at, d));
@@ -226,7 +237,7 @@ __global__ __launch_bounds__(kThreads) void verify_argmax_kernel(TreeVerifyParam
 }
 
 // A row's largest logit and its sum of weights relative to it, by one wave.
-__device__ __forceinline__ void row_stats(const TreeVerifyParams& p, const double* table, int side, int t, int lane, float& m,
+__device__ __forceinline__ void row_stats(const TreeVerifyParams& p, const unsigned long long* table, int side, int t, int lane, float& m,
                                           double& z) {
   const long long at = ((long long)side * p.nodes + t) * p.groups;
   const bool first = lane < p.groups;                  // the lane's first group, loaded once
@@ -248,7 +259,7 @@ __device__ __forceinline__ double row16_sum64(double x) {
   return x;
 }
 // (With weight_call: only the one-workgroup kernel uses it.)
-__device__ __forceinline__ void row_stats16(const TreeVerifyParams& p, const double* table, int side, int t, int c, float& m,
+__device__ __forceinline__ void row_stats16(const TreeVerifyParams& p, const unsigned long long* table, int side, int t, int c, float& m,
                                             double& z) {
   const long long at = ((long long)side * p.nodes + t) * p.groups;
   float mc[2];                                         // the lane's first two groups, loaded once
@@ -290,7 +301,7 @@ struct Residual {
 __device__ __forceinline__ void reject(const TreeVerifyParams& p, int t, int rejected, int lane, Residual& r) {
   if (r.round != rejected - 1) return;
   const double s = round_total(p, rejected, t, lane);
-  if (s > 0.0) r = Residual{r.a + r.s, s, rejected};
+  if (s > kNothing) r = Residual{r.a + r.s, s, rejected};
 }
 
 __device__ __forceinline__ float logit(const uint16_t* row, int v) {
@@ -298,19 +309,18 @@ __device__ __forceinline__ float logit(const uint16_t* row, int v) {
 }
 // Probability of token x in a row; 0 outside the vocabulary.
 __device__ __forceinline__ double probability(const uint16_t* row, int x, int vocab, const Scale& s, double z,
-                                              const double* table) {
+                                              const unsigned long long* table) {
   return x >= 0 && x < vocab ? weight(logit(row, x), s, table) / z : 0.0;
 }
 
 // (2) Round `round` of drawn drafts: blockIdx = (chunk, node).  Each wave finds out for itself
 // whether the node's first `round` children are all rejected; the chunk's logits are under way
 // meanwhile.
-template <int kRuns>
 __global__ __launch_bounds__(kThreads) void verify_round_kernel(TreeVerifyParams p, int round) {
-  __shared__ double table[32];
-  __shared__ double ss[kRuns][kThreads / 64];
+  __shared__ unsigned long long table[32];
+  __shared__ double ss[kVerifyRuns][kWaves];
   load_arguments(p);
-  const int t = blockIdx.y, c = blockIdx.x * kRuns, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int t = blockIdx.y, c = blockIdx.x * p.runs, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint16_t* rp = p.target + t * p.ldt;
   const uint16_t* rq = p.draft + t * p.ldd;
   int child = -1, found = 0;                           // lane k: the node's child k (from 0), k < round
@@ -321,14 +331,9 @@ __global__ __launch_bounds__(kThreads) void verify_round_kernel(TreeVerifyParams
       if (lane == found) child = s0 + __builtin_ctzll(hits);
   }
   if (found < round) return;                           // the same in every wave
-  load_table(table);
+  if (threadIdx.x < 32) table[threadIdx.x] = kPow32[threadIdx.x];
   const int v0 = c * kVerifyChunk + 8 * threadIdx.x;
-  float x[kRuns][8], y[kRuns][8];
-#pragma unroll
-  for (int i = 0; i < kRuns; ++i) {
-    load8(rp, v0 + kVerifyChunk * i, p.vocab, x[i]);
-    load8(rq, v0 + kVerifyChunk * i, p.vocab, y[i]);
-  }
+  f16x8u xr = fetch8(rp, v0, p.vocab), yr = fetch8(rq, v0, p.vocab);
   __syncthreads();
   float mp, mq;
   double zp, zq;
@@ -349,14 +354,20 @@ __global__ __launch_bounds__(kThreads) void verify_round_kernel(TreeVerifyParams
     if (k + 1 < round) reject(p, t, k + 1, lane, r);
   }
   const double a = (r.a + r.s) / zq, ip = 1.0 / zp;
-#pragma unroll
-  for (int i = 0; i < kRuns; ++i) {
+#pragma unroll 1
+  for (int i = 0; i < p.runs; ++i) {
     double s = 0.0;
+    const int v = v0 + kVerifyChunk * i;
+    const f16x8u xc = xr, yc = yr;
+    xr = fetch8(rp, v + kVerifyChunk, p.vocab);
+    yr = fetch8(rq, v + kVerifyChunk, p.vocab);
     if (r.round == round - 1) {                        // else an earlier round's sum was 0
-      const int v = v0 + kVerifyChunk * i;
+      float x[8], y[8];
       double wp[8], wq[8];
-      weights8(x[i], v, p.vocab, sp, table, wp);
-      weights8(y[i], v, p.vocab, sq, table, wq);
+      expand8(xc, rp, v, p.vocab, x);
+      expand8(yc, rq, v, p.vocab, y);
+      weights8(x, v, p.vocab, sp, table, wp);
+      weights8(y, v, p.vocab, sq, table, wq);
 #pragma unroll
       for (int e = 0; e < 8; ++e) s += fmax(wp[e] * ip - wq[e] * a, 0.0);
     }
@@ -364,7 +375,7 @@ __global__ __launch_bounds__(kThreads) void verify_round_kernel(TreeVerifyParams
     if (lane == 0) ss[i][wave] = s;
   }
   __syncthreads();
-  if (threadIdx.x < kRuns && c + (int)threadIdx.x < p.chunks) {
+  if ((int)threadIdx.x < p.runs && c + (int)threadIdx.x < p.chunks) {
     double s = ss[threadIdx.x][0];
     for (int w = 1; w < kThreads / 64; ++w) s += ss[threadIdx.x][w];
     p.rounds[((long long)(round - 1) * p.nodes + t) * p.chunks + c + threadIdx.x] = s;
@@ -377,7 +388,7 @@ constexpr int kWalkWaves = kWalkThreads / 64;
 constexpr int kMaxChunks = (1 << 24) / kVerifyChunk;   // of the largest vocabulary
 
 struct WalkShared {
-  double table[32];
+  unsigned long long table[32];
   int parent[kNodes], token[kNodes], next[kNodes], path[kNodes], best[kNodes];
   float mp[kNodes], mq[kNodes], u[kNodes];
   double zp[kNodes], zq[kNodes];
@@ -408,7 +419,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const bool drawn = !p.greedy && p.draft != nullptr;
   const float sample_u = p.greedy ? 0.0f : *p.sample_u;
-  if (!p.greedy) load_table(sh.table);
+  if (!p.greedy && tid < 32) sh.table[tid] = kPow32[tid];
   for (int t = tid; t < p.nodes; t += kWalkThreads) {
     const int parent = t ? p.parents[t] : -1;
     sh.parent[t] = parent < t ? parent : -1;           // otherwise never reached
@@ -562,7 +573,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
           if (sh.parent[k] == node && sh.token[k] >= 0 && sh.token[k] / kVerifyChunk == c) s -= sh.pw[k];
         if (s < 1e-3 * all) s = -1.0;                  // to be summed again
       }
-      sums[c] = s;
+      sums[c] = s >= 0.0 && s < kNothing ? 0.0 : s;
     }
     __syncthreads();
     if (holes)
@@ -664,25 +675,17 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
   if (tid == 0) *p.count = count;
 }
 
-template <int kRuns>
-void launch_passes(const TreeVerifyParams& p, hipStream_t stream) {
-  if (p.greedy) {
-    hipLaunchKernelGGL(verify_argmax_kernel<kRuns>, dim3(p.groups, p.nodes), dim3(kThreads), 0, stream, p);
-    return;
-  }
-  hipLaunchKernelGGL(verify_stats_kernel<kRuns>, dim3(p.groups, p.nodes, p.draft ? 2 : 1), dim3(kThreads), 0, stream, p);
-  if (p.draft)
-    for (int r = 1; r <= p.max_children; ++r)
-      hipLaunchKernelGGL(verify_round_kernel<kRuns>, dim3(p.groups, p.nodes), dim3(kThreads), 0, stream, p, r);
-}
-
 }  // namespace
 
 hipError_t launch_tree_verify(const TreeVerifyParams& p, hipStream_t stream) {
-  if (p.runs == 4)
-    launch_passes<4>(p, stream);
-  else
-    launch_passes<1>(p, stream);
+  if (p.greedy) {
+    hipLaunchKernelGGL(verify_argmax_kernel, dim3(p.groups, p.nodes), dim3(kThreads), 0, stream, p);
+  } else {
+    hipLaunchKernelGGL(verify_stats_kernel, dim3(p.groups, p.nodes, p.draft ? 2 : 1), dim3(kThreads), 0, stream, p);
+    if (p.draft)
+      for (int r = 1; r <= p.max_children; ++r)
+        hipLaunchKernelGGL(verify_round_kernel, dim3(p.groups, p.nodes), dim3(kThreads), 0, stream, p, r);
+  }
   hipLaunchKernelGGL(verify_walk_kernel, dim3(1), dim3(kWalkThreads), 0, stream, p);
   return hipGetLastError();
 }
