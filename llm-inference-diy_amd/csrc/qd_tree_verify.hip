@@ -41,15 +41,13 @@ __device__ __forceinline__ void load_arguments(const TreeVerifyParams& p) {
 }
 
 // Weight of a logit in a row (or chunk): `m` its largest logit, `scale` 32 log2(e) / temperature
-// (exponents are counted in 32nds), `least` the smallest logit that still has one.
+// (exponents are counted in 32nds).
 struct Scale {
-  float m, least;
+  float m;
   double md, scale;
 };
-constexpr double kLeast = 28800.0;                     // 2^-900
-__device__ __forceinline__ Scale make_scale(float m, double scale) {
-  return Scale{m, m - (float)(kLeast / scale), (double)m, scale};
-}
+__device__ __forceinline__ Scale make_scale(float m, double scale) { return Scale{m, (double)m, scale}; }
+constexpr double kLeast = -28800.0;                    // 2^-900
 // What a sum may hold of weights that should be 0 (2^24 of 2^-900) counts as 0.
 constexpr double kNothing = 1e-250;
 
@@ -66,15 +64,14 @@ __device__ const unsigned long long kPow32[32] = {
     0x3fef5818dcfba487, 0x3fef7c97337b9b5f, 0x3fefa4afa2a490da, 0x3fefd0765b6e4540,
 };
 
-// 2^(x / 32), x = (l - m) * scale <= 0, to a relative 2e-12: 2^(n/32) times the series of 2^(f/32)
-// to degree 4 on |f| <= 1/2 (remainder (ln2/64)^5 / 5! = 1.3e-12; the difference of two halves is
-// exact).  Rounding to n by adding 1.5 * 2^52 leaves it in the low word.  A NaN, and whatever
-// weighs less than 2^-900, counts as 2^-900.  m is finite.  The passes are bound by the number
-// of instructions, of which this takes 16 (fp64 ones issue at the fp32 rate): KSTATS.
+// 2^(x / 32), kLeast <= x <= 0, to a relative 2e-12: 2^(n/32) times the series of 2^(f/32)
+// to degree 4 on |f| <= 1/2 (remainder (ln2/64)^5 / 5! = 1.3e-12).
+// Rounding to n by adding 1.5 * 2^52 leaves it in the low word.  (A series on |f| <= 1/2 of a whole
+// exponent, without the table, takes six fp64 instructions more: the pass over 64 rows of 151936
+// logits 14.2 us against 13.9.)
 // table: the workgroup's copy of kPow32 in LDS, 256 bytes: one entry per pair of banks, so
 // lanes never conflict.
-__device__ __forceinline__ double weight_finite(float l, const Scale& s, const unsigned long long* table) {
-  const double x = ((double)fmaxf(l, s.least) - s.md) * s.scale;
+__device__ __forceinline__ double exp2_32nds(double x, const unsigned long long* table) {
   const double t = x + 0x1.8p52;
   const double f = x - (t - 0x1.8p52);
   const unsigned n = (unsigned)__builtin_bit_cast(unsigned long long, t);
@@ -86,10 +83,18 @@ __device__ __forceinline__ double weight_finite(float l, const Scale& s, const u
   r = __builtin_fma(r, f, 0.02166084939249829);
   return __builtin_fma(base, r * f, base);
 }
-// The same for any m, and 0 where there is no weight: the largest logits weigh 1 also where they
-// are infinite.
+// The weight where m is finite, for sums: a NaN, and what weighs less than 2^-900, counts as
+// 2^-900.  (The difference of two halves is exact.)
+__device__ __forceinline__ double weight_finite(float l, const Scale& s, const unsigned long long* table) {
+  return exp2_32nds(fmax(((double)l - s.md) * s.scale, kLeast), table);
+}
+// For any m, and 0 where there is no weight: the largest logits weigh 1 also where they are
+// infinite.
 __device__ __forceinline__ double weight(float l, const Scale& s, const unsigned long long* table) {
-  if (fabsf(s.m) < __builtin_inff()) return l > s.least ? weight_finite(l, s, table) : 0.0;
+  if (fabsf(s.m) < __builtin_inff()) {
+    const double x = ((double)l - s.md) * s.scale;
+    return x > kLeast ? exp2_32nds(x, table) : 0.0;    // 0 where x is NaN, too
+  }
   if (l != l) l = -__builtin_inff();
   return l == s.m ? 1.0 : 0.0;
 }

@@ -241,6 +241,23 @@ def test_temperatures(qdiy, mode, temperature):
     c.check(qdiy)
 
 
+@pytest.mark.parametrize("mode", ["point", "drawn"])
+@pytest.mark.parametrize("temperature", [1e-6, 1e-3, 100.0])
+def test_large_logits(qdiy, mode, temperature):
+    """Logits near the ends of their type: neighbours differ by 32, far more than the temperature."""
+    c = Case(9, 3000, "point", seed=2)
+    rng = np.random.default_rng(12)
+    c.mode, c.temperature = mode, temperature
+    c.logits = (rng.standard_normal((9, 3000)) * 20000).clip(-65000, 65000).astype(np.float16)
+    c.logits[:, 7] = np.float16(65504)
+    c.logits[:, 1500] = np.float16(65472)
+    if mode == "drawn":
+        c.draft = c.logits.copy()
+        c.draft[:, 1500] = np.float16(65504)
+    c.tokens[1:] = np.where(rng.random(8) < 0.5, 7, 1500)
+    c.check(qdiy)
+
+
 @pytest.mark.parametrize("mode", MODES)
 def test_captured_and_replayed(qdiy, mode):
     c = Case(27, 9000, mode, seed=0)
