@@ -553,11 +553,26 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
       float x[8], y[8];
       load8(rp, v, p.vocab, x);
       if (rq) load8(rq, v, p.vocab, y);
+      if (fabsf(mp) < __builtin_inff() && fabsf(mq) < __builtin_inff()) {   // eight at once
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = v + e < p.vocab ? weight_call(x[e], mp, p.scale_log2, sh.table) * ip : 0.0;
-      if (rq) {
+        for (int e = 0; e < 8; ++e) {
+          const double d = ((double)x[e] - (double)mp) * p.scale_log2;
+          w[e] = d > kLeast ? exp2_32nds(d, sh.table) * ip : 0.0;   // past the row's end: -inf
+        }
+        if (rq) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = fmax(w[e] - weight_call(y[e], mq, p.scale_log2, sh.table) * a, 0.0);
+          for (int e = 0; e < 8; ++e) {
+            const double d = ((double)y[e] - (double)mq) * p.scale_log2;
+            w[e] = fmax(w[e] - (d > kLeast ? exp2_32nds(d, sh.table) * a : 0.0), 0.0);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (v + e < p.vocab) {
+            w[e] = weight_call(x[e], mp, p.scale_log2, sh.table) * ip;
+            if (rq) w[e] = fmax(w[e] - weight_call(y[e], mq, p.scale_log2, sh.table) * a, 0.0);
+          }
       }
       if (holes) {
         const unsigned gone = (sh.gone[i0 >> 5] >> (i0 & 31)) & 0xffu;

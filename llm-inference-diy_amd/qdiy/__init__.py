@@ -659,7 +659,7 @@ def tree_layout(parents) -> tuple:
     """qd_tree_layout: (mask int64 [nodes][ceil(nodes / 64)], depth int32 [nodes]) of a drafted
     tree as CPU tensors; parents[0] is negative, parents[t] < t."""
     n = len(parents)
-    par = (ctypes.c_int * max(1, n))(*parents)
+    par = (ctypes.c_int * max(1, n))(*map(int, parents))
     mask = torch.empty((n, (n + 63) // 64), dtype=torch.int64)
     depth = torch.empty(n, dtype=torch.int32)
     _check(load().qd_tree_layout(par, n, ctypes.cast(mask.data_ptr(), ctypes.POINTER(ctypes.c_uint64)),
