@@ -5,8 +5,7 @@
 // their sums, and the residuals max(p - A q, 0).  A decision compares a random
 // number with a ratio of such sums, and the last token is the first index whose
 // cumulative weight passes a random share of the total: with a vocabulary of
-// 150 thousand, fp32 sums would move the chosen index.  (fp64 fused multiply-adds
-// issue at the fp32 rate on this part, so this costs little.)
+// 150 thousand, fp32 sums would move the chosen index.
 //
 // Residuals of drawn drafts in closed form: with p normalised, A_0 = 0, S_0 = 1,
 // the distribution after j rejections is max(p - A_j q, 0) / S_j, where
@@ -18,7 +17,12 @@
 // chunks' sums of S_j, for every node whose first j children are all rejected; (3) one
 // workgroup reduces the rows' partials, decides every node's children (a node's decisions do
 // not depend on how it was reached), walks from node 0, and takes the last token from one
-// chunk.
+// chunk.  A single pass cannot do: p needs its row's whole sum, and S_j the sums before it.
+//
+// Measured on MI355X: 64 rows of 151936 logits 13 us (25 instructions per logit are 15 of its 25
+// thousand cycles; the loads' and LDS latency at its two ends the rest) and the one workgroup
+// 15; 27 rows of drawn drafts over 32003 logits 5, four rounds of 3.6-6.8 and 14; the greedy
+// check of 5 rows 3.7 and 4.0.
 #include "qd_device.h"
 #include "qd_internal.h"
 #include "qd_tree.h"
