@@ -96,8 +96,8 @@ inline TreeAttnPlan tree_attn_plan(int nodes, int heads, int kv_heads, int prefi
 hipError_t launch_tree_attention(const TreeAttnParams& p, const TreeAttnPlan& plan, hipStream_t stream);
 
 // Logits of a row per chunk of the verification's passes, and chunks per workgroup: as many as
-// leave two workgroups per CU (more would be dispatched one after the other, fewer leave CUs
-// empty: 5 rows of 151936 logits, argmax pass, 3.8 us at 1 chunk, 5.8 at 4), at most 16.
+// leave four workgroups per CU (5 rows of 151936 logits, argmax pass, 3.8 us at 1 chunk, 5.8 at
+// 4, which leaves CUs empty; 64 rows, sums of weights, 14.7 us at 1, 14.1 at 4), at most 16.
 constexpr int kVerifyChunk = 2048;
 constexpr int kVerifyRuns = 16;
 inline int verify_runs(int nodes, int chunks) {

@@ -493,8 +493,9 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
         if (p.greedy) {
           ok = sh.token[s] == sh.best[t];
         } else if (!drawn) {
+          left = fmax(left, sh.pw[s]);                 // rounding may have taken a little of the token's own share
           ok = (double)sh.u[s] * left < sh.pw[s];
-          left = fmax(left - sh.pw[s], 0.0);
+          left -= sh.pw[s];
         } else {
           if (rejected == p.max_children) break;
           ok = (double)sh.u[s] * sh.qw[s] * r.s < fmax(sh.pw[s] - r.a * sh.qw[s], 0.0);

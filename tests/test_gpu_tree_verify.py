@@ -304,3 +304,16 @@ def test_a_vocabulary_of_many_chunks(qdiy, mode):
     """More chunks than a wave's lanes, in the short and in the long chunks."""
     Case(2, 300001, mode, seed=2, parents=[-1, 0]).check(qdiy)
     Case(3, 4500000, mode, seed=3, parents=[-1, 0, 0]).check(qdiy)
+
+
+def test_rejected_by_a_random_number_of_one(qdiy):
+    """u = 1 rejects every child of a point draft, also where one token holds all but 1e-17 of
+    the weight, so that nothing representable is left of 1 after it."""
+    c = Case(5, 300, "point", seed=9, parents=[-1, 0, 0, 0, 1], temperature=1.0)
+    c.logits[:] = np.float16(0.0)
+    c.logits[:, 7] = np.float16(45.0)
+    c.logits[:, 11] = np.float16(3.0)
+    c.tokens[1:] = [7, 11, 12, 7]
+    c.au[:] = 1.0
+    path, out = c.check(qdiy)
+    assert path == [0] and out[0] not in (7, 11, 12)
