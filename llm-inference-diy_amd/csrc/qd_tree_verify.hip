@@ -108,10 +108,51 @@ __device__ __attribute__((noinline)) double weight_call(float l, float m, double
   return weight(l, make_scale(m, scale), table);
 }
 
-__device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+// Reductions and scans by row operations and lane reads; every lane has to be there.  (Shuffles
+// go through LDS, at some 100 cycles a step and two of them for 64 bits: the four rounds over 27
+// rows of 32003 logits took 6.0 to 7.1 us with them, 5.3 to 6.4 without, the one-workgroup
+// kernel 12.9 and 10.9.)
+template <int Ctrl>
+__device__ __forceinline__ double dpp_mov64(double x) {
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, x);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)b, Ctrl, 0xF, 0xF, true);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), Ctrl, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+// The value of lane `at`, which is the same in all lanes.
+__device__ __forceinline__ float lane_value(float x, int at) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), at));
+}
+__device__ __forceinline__ double lane_value(double x, int at) {
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, x);
+  const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)b, at), hi = __builtin_amdgcn_readlane((int)(b >> 32), at);
+  return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+// Over the 16 lanes of a row; all of them receive it.
+__device__ __forceinline__ double row16_sum64(double x) {
+  x += dpp_mov64<kDppQuadSwap1>(x);
+  x += dpp_mov64<kDppQuadSwap2>(x);
+  x += dpp_mov64<kDppHalfMirror>(x);
+  x += dpp_mov64<kDppMirror>(x);
   return x;
+}
+__device__ __forceinline__ double wave_sum(double x) {
+  x = row16_sum64(x);
+  return (lane_value(x, 0) + lane_value(x, 16)) + (lane_value(x, 32) + lane_value(x, 48));
+}
+__device__ __forceinline__ float wave_max(float x) {
+  x = row16_max(x);
+  return fmaxf(fmaxf(lane_value(x, 0), lane_value(x, 16)), fmaxf(lane_value(x, 32), lane_value(x, 48)));
+}
+// Inclusive.  Lanes without a partner to the left add 0.
+__device__ __forceinline__ double wave_scan(double x, int lane) {
+  x += dpp_mov64<0x111>(x);                            // row_shr:1, 2, 4, 8
+  x += dpp_mov64<0x112>(x);
+  x += dpp_mov64<0x114>(x);
+  x += dpp_mov64<0x118>(x);
+  const double r0 = lane_value(x, 15), r1 = r0 + lane_value(x, 31), r2 = r1 + lane_value(x, 47);
+  const double before = lane < 32 ? (lane < 16 ? 0.0 : r0) : lane < 48 ? r1 : r2;
+  return x + before;
 }
 
 // Eight logits from index v on; -inf past the row's end.  In two steps, so that several runs'
@@ -177,7 +218,7 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(TreeVerifyParams
     expand8(cur, row, v, p.vocab, x);
 #pragma unroll
     for (int e = 0; e < 8; ++e) m = fmaxf(m, x[e]);    // fmaxf passes NaN over
-    m = wave64_max(m);
+    m = wave_max(m);
     weights8(x, v, p.vocab, make_scale(m, p.scale_log2), table, w);
     const double s = wave_sum(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
     if (lane == 0) {
@@ -188,10 +229,11 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(TreeVerifyParams
   __syncthreads();
   if (wave == 0) {
     const int parts = p.runs * kWaves;
-    const float m = lane < parts ? sm[lane] : -__builtin_inff(), mg = wave64_max(m);
+    const float m = lane < parts ? sm[lane] : -__builtin_inff(), mg = wave_max(m);
     double s = lane < parts ? ss[lane] * weight(m, make_scale(mg, p.scale_log2), table) : 0.0;
-#pragma unroll
-    for (int d = 1; d < kWaves; d <<= 1) s += __shfl_xor(s, d);   // the run's, in each of its lanes
+    static_assert(kWaves == 4, "a run's parts are four lanes");
+    s += dpp_mov64<kDppQuadSwap1>(s);
+    s += dpp_mov64<kDppQuadSwap2>(s);                  // the run's, in each of its lanes
     const double all = wave_sum(lane % kWaves == 0 ? s : 0.0);    // 0 past the row's end
     const long long row_at = (long long)side * p.nodes + t;
     if (lane % kWaves == 0 && lane < parts && c + lane / kWaves < p.chunks) p.sums[row_at * p.chunks + c + lane / kWaves] = s;
@@ -245,58 +287,66 @@ __global__ __launch_bounds__(kThreads) void verify_argmax_kernel(TreeVerifyParam
   }
 }
 
-// A row's largest logit and its sum of weights relative to it, by one wave.
-__device__ __forceinline__ void row_stats(const TreeVerifyParams& p, const unsigned long long* table, int side, int t, int lane, float& m,
-                                          double& z) {
-  const long long at = ((long long)side * p.nodes + t) * p.groups;
-  const bool first = lane < p.groups;                  // the lane's first group, loaded once
-  const float m0 = first ? p.maxes[at + lane] : -__builtin_inff();
-  const double s0 = first ? p.group_sums[at + lane] : 0.0;
-  m = m0;
-  for (int c = lane + 64; c < p.groups; c += 64) m = fmaxf(m, p.maxes[at + c]);
-  m = wave64_max(m);
-  const Scale sc = make_scale(m, p.scale_log2);
-  z = first ? s0 * weight(m0, sc, table) : 0.0;
-  for (int c = lane + 64; c < p.groups; c += 64) z += p.group_sums[at + c] * weight(p.maxes[at + c], sc, table);
-  z = wave_sum(z);
-}
-
-// The same by 16 lanes (four rows per wave at once).
-__device__ __forceinline__ double row16_sum64(double x) {
-#pragma unroll
-  for (int d = 8; d; d >>= 1) x += __shfl_xor(x, d);
-  return x;
-}
-// (With weight_call: only the one-workgroup kernel uses it.)
-__device__ __forceinline__ void row_stats16(const TreeVerifyParams& p, const unsigned long long* table, int side, int t, int c, float& m,
-                                            double& z) {
-  const long long at = ((long long)side * p.nodes + t) * p.groups;
-  float mc[2];                                         // the lane's first two groups, loaded once
-  double sc[2];
+// A row's groups as 16 lanes load them, two each, and from them and the rest of a long row its
+// largest logit and its sum of weights relative to it.  In two steps, so that other loads are in
+// flight with these.  The rounds and the one-workgroup kernel form both alike, so that they take
+// the same decisions.
+struct Groups {
+  long long at;
+  float m[2];
+  double s[2];
+};
+__device__ __forceinline__ Groups fetch_groups(const TreeVerifyParams& p, int side, int t, int c) {
+  Groups g;
+  g.at = ((long long)side * p.nodes + t) * p.groups;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const bool in = c + 16 * i < p.groups;
-    mc[i] = in ? p.maxes[at + c + 16 * i] : -__builtin_inff();
-    sc[i] = in ? p.group_sums[at + c + 16 * i] : 0.0;
+    g.m[i] = in ? p.maxes[g.at + c + 16 * i] : -__builtin_inff();
+    g.s[i] = in ? p.group_sums[g.at + c + 16 * i] : 0.0;
   }
-  m = fmaxf(mc[0], mc[1]);
-  for (int i = c + 32; i < p.groups; i += 16) m = fmaxf(m, p.maxes[at + i]);
+  return g;
+}
+__device__ __forceinline__ void row_stats(const TreeVerifyParams& p, const unsigned long long* table, const Groups& g, int c, float& m,
+                                          double& z) {
+  m = fmaxf(g.m[0], g.m[1]);
+#pragma unroll 4
+  for (int i = c + 32; i < p.groups; i += 16) m = fmaxf(m, p.maxes[g.at + i]);
   m = row16_max(m);
   z = 0.0;
+  float m0 = g.m[0], m1 = g.m[1];
+  double s0 = g.s[0], s1 = g.s[1];
 #pragma unroll 1
-  for (int i = c; i < p.groups; i += 16) {
-    const float mi = i == c ? mc[0] : i == c + 16 ? mc[1] : p.maxes[at + i];
-    const double si = i == c ? sc[0] : i == c + 16 ? sc[1] : p.group_sums[at + i];
-    z += si * weight_call(mi, m, p.scale_log2, table);
+  for (int i = 0; i < p.groups; i += 16) {             // the same for all lanes
+    const bool in = i + c + 32 < p.groups;
+    const float m2 = in ? p.maxes[g.at + i + c + 32] : -__builtin_inff();
+    const double s2 = in ? p.group_sums[g.at + i + c + 32] : 0.0;
+    z += s0 * weight_call(m0, m, p.scale_log2, table);
+    m0 = m1;
+    s0 = s1;
+    m1 = m2;
+    s1 = s2;
   }
   z = row16_sum64(z);
 }
 
+// The first 64 chunks' sums of a node's rounds 1 to 3, a chunk per lane, loaded before it is
+// known which will be needed (of rounds that are not: whatever is there).
+struct Ahead {
+  double r1, r2, r3;
+};
+__device__ __forceinline__ Ahead fetch_rounds(const TreeVerifyParams& p, int rounds, int t, int lane) {
+  const double* s = p.rounds + (long long)t * p.chunks + lane;
+  const long long next = (long long)p.nodes * p.chunks;
+  const bool in = lane < p.chunks;
+  return Ahead{in && rounds > 0 ? s[0] : 0.0, in && rounds > 1 ? s[next] : 0.0, in && rounds > 2 ? s[2 * next] : 0.0};
+}
 // The sum over chunks of round r (from 1) of node t, by one wave.
-__device__ __forceinline__ double round_total(const TreeVerifyParams& p, int r, int t, int lane) {
+__device__ __forceinline__ double round_total(const TreeVerifyParams& p, int r, int t, int lane, const Ahead& first) {
   const double* s = p.rounds + ((long long)(r - 1) * p.nodes + t) * p.chunks;
-  double z = 0.0;
-  for (int c = lane; c < p.chunks; c += 64) z += s[c];
+  double z = r == 1 ? first.r1 : r == 2 ? first.r2 : first.r3;
+  if (r > 3) z = lane < p.chunks ? s[lane] : 0.0;
+  for (int c = lane + 64; c < p.chunks; c += 64) z += s[c];
   return wave_sum(z);
 }
 
@@ -307,24 +357,18 @@ struct Residual {
   double a, s;
   int round;
 };
-__device__ __forceinline__ void reject(const TreeVerifyParams& p, int t, int rejected, int lane, Residual& r) {
+__device__ __forceinline__ void reject(const TreeVerifyParams& p, int t, int rejected, int lane, const Ahead& first, Residual& r) {
   if (r.round != rejected - 1) return;
-  const double s = round_total(p, rejected, t, lane);
+  const double s = round_total(p, rejected, t, lane, first);
   if (s > kNothing) r = Residual{r.a + r.s, s, rejected};
 }
 
 __device__ __forceinline__ float logit(const uint16_t* row, int v) {
   return (float)reinterpret_cast<const _Float16*>(row)[v];
 }
-// Probability of token x in a row; 0 outside the vocabulary.
-__device__ __forceinline__ double probability(const uint16_t* row, int x, int vocab, const Scale& s, double z,
-                                              const unsigned long long* table) {
-  return x >= 0 && x < vocab ? weight(logit(row, x), s, table) / z : 0.0;
-}
-
 // (2) Round `round` of drawn drafts: blockIdx = (chunk, node).  Each wave finds out for itself
-// whether the node's first `round` children are all rejected; the chunk's logits are under way
-// meanwhile.
+// whether the node's first `round` children are all rejected; all that it takes for that but
+// the children's tokens and their logits, and the chunk's logits, is loaded at once.
 __global__ __launch_bounds__(kThreads) void verify_round_kernel(TreeVerifyParams p, int round) {
   __shared__ unsigned long long table[32];
   __shared__ double ss[kVerifyRuns][kWaves];
@@ -332,6 +376,8 @@ __global__ __launch_bounds__(kThreads) void verify_round_kernel(TreeVerifyParams
   const int t = blockIdx.y, c = blockIdx.x * p.runs, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint16_t* rp = p.target + t * p.ldt;
   const uint16_t* rq = p.draft + t * p.ldd;
+  const Groups g = fetch_groups(p, (lane >> 4) & 1, t, lane & 15);   // target and drafter, twice
+  const Ahead first = fetch_rounds(p, round - 1, t, lane);
   int child = -1, found = 0;                           // lane k: the node's child k (from 0), k < round
   for (int s0 = t + 1; s0 < p.nodes && found < round; s0 += 64) {
     const int s = s0 + lane;
@@ -340,27 +386,26 @@ __global__ __launch_bounds__(kThreads) void verify_round_kernel(TreeVerifyParams
       if (lane == found) child = s0 + __builtin_ctzll(hits);
   }
   if (found < round) return;                           // the same in every wave
-  if (threadIdx.x < 32) table[threadIdx.x] = kPow32[threadIdx.x];
   const int v0 = c * kVerifyChunk + 8 * threadIdx.x;
+  const int tok = child >= 0 ? p.tokens[child] : -1;
+  const float u = child >= 0 ? p.accept_u[child] : 0.0f;
   f16x8u xr = fetch8(rp, v0, p.vocab), yr = fetch8(rq, v0, p.vocab);
+  if (threadIdx.x < 32) table[threadIdx.x] = kPow32[threadIdx.x];
+  const bool in = tok >= 0 && tok < p.vocab;
+  const float lp = in ? logit(rp, tok) : 0.0f, lq = in ? logit(rq, tok) : 0.0f;
   __syncthreads();
-  float mp, mq;
-  double zp, zq;
-  row_stats(p, table, 0, t, lane, mp, zp);
-  row_stats(p, table, 1, t, lane, mq, zq);
+  float m;
+  double z;
+  row_stats(p, table, g, lane & 15, m, z);
+  const float mp = lane_value(m, 0), mq = lane_value(m, 16);
+  const double zp = lane_value(z, 0), zq = lane_value(z, 16);
   const Scale sp = make_scale(mp, p.scale_log2), sq = make_scale(mq, p.scale_log2);
-  double pw = 0.0, uq = 0.0, qw = 0.0;
-  if (child >= 0) {
-    const int tok = p.tokens[child];
-    pw = probability(rp, tok, p.vocab, sp, zp, table);
-    qw = probability(rq, tok, p.vocab, sq, zq, table);
-    uq = (double)p.accept_u[child] * qw;
-  }
+  const double pw = in ? weight(lp, sp, table) / zp : 0.0, qw = in ? weight(lq, sq, table) / zq : 0.0, uq = (double)u * qw;
   Residual r{0.0, 1.0, 0};
   for (int k = 0; k < round; ++k) {
-    const bool ok = __shfl(uq, k) * r.s < fmax(__shfl(pw, k) - r.a * __shfl(qw, k), 0.0);
+    const bool ok = lane_value(uq, k) * r.s < fmax(lane_value(pw, k) - r.a * lane_value(qw, k), 0.0);
     if (ok) return;                                    // a child stands: no later round is looked at
-    if (k + 1 < round) reject(p, t, k + 1, lane, r);
+    if (k + 1 < round) reject(p, t, k + 1, lane, first, r);
   }
   const double a = (r.a + r.s) / zq, ip = 1.0 / zp;
 #pragma unroll 1
@@ -398,9 +443,10 @@ constexpr int kMaxChunks = (1 << 24) / kVerifyChunk;   // of the largest vocabul
 
 struct WalkShared {
   unsigned long long table[32];
-  int parent[kNodes], token[kNodes], next[kNodes], path[kNodes], best[kNodes];
+  int parent[kNodes], token[kNodes], next[kNodes], path[kNodes], best[kNodes], round[kNodes];
   float mp[kNodes], mq[kNodes], u[kNodes];
   double zp[kNodes], zq[kNodes];
+  double a[kNodes], s[kNodes];                         // with round: what a node's children left, if all are rejected
   double pw[kNodes], qw[kNodes];                       // a node's token in its parent's distributions
   double wave[kWalkWaves];
   unsigned gone[kVerifyChunk / 32];                       // rejected tokens of one chunk
@@ -429,12 +475,23 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
   const bool drawn = !p.greedy && p.draft != nullptr;
   const float sample_u = p.greedy ? 0.0f : *p.sample_u;
   if (!p.greedy && tid < 32) sh.table[tid] = kPow32[tid];
-  for (int t = tid; t < p.nodes; t += kWalkThreads) {
-    const int parent = t ? p.parents[t] : -1;
-    sh.parent[t] = parent < t ? parent : -1;           // otherwise never reached
-    sh.token[t] = t ? p.tokens[t] : -1;
-    sh.u[t] = t && !p.greedy ? p.accept_u[t] : 0.0f;
-    sh.next[t] = -1;
+  // Thread t: node t and, on their way while the rows are summed, its token's logits in its
+  // parent's rows.
+  static_assert(kWalkThreads >= kNodes, "a thread per node");
+  int parent = -1, token = -1;
+  float lp = 0.0f, lq = 0.0f;
+  if (tid < p.nodes) {
+    const int above = tid ? p.parents[tid] : -1;
+    parent = above < tid ? above : -1;                 // otherwise never reached
+    token = tid ? p.tokens[tid] : -1;
+    sh.u[tid] = tid && !p.greedy ? p.accept_u[tid] : 0.0f;
+    sh.parent[tid] = parent;
+    sh.token[tid] = token;
+  }
+  const bool in = !p.greedy && parent >= 0 && token >= 0 && token < p.vocab;
+  if (in) {
+    lp = logit(p.target + parent * p.ldt, token);
+    if (drawn) lq = logit(p.draft + parent * p.ldd, token);
   }
   __syncthreads();
   for (int t0 = 4 * wave; t0 < p.nodes; t0 += 4 * kWalkWaves) {   // four rows per wave, 16 lanes each
@@ -450,8 +507,9 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
     } else {
       float m, mq = 0.0f;
       double z, zq = 1.0;
-      row_stats16(p, sh.table, 0, t, c0, m, z);
-      if (drawn) row_stats16(p, sh.table, 1, t, c0, mq, zq);     // of a node without children: not written, not used
+      const Groups gp = fetch_groups(p, 0, t, c0), gq = drawn ? fetch_groups(p, 1, t, c0) : Groups{};
+      row_stats(p, sh.table, gp, c0, m, z);
+      if (drawn) row_stats(p, sh.table, gq, c0, mq, zq);     // of a node without children: not written, not used
       if (c0 == 0) {
         sh.mp[t] = m;
         sh.zp[t] = z;
@@ -462,20 +520,19 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
   }
   __syncthreads();
   if (!p.greedy) {
-    for (int s = tid; s < p.nodes; s += kWalkThreads) {
-      const int t = sh.parent[s], x = sh.token[s];
+    if (tid < p.nodes) {
       double pw = 0.0, qw = 0.0;
-      if (t >= 0) {
-        const bool in = x >= 0 && x < p.vocab;
-        const float lp = in ? logit(p.target + t * p.ldt, x) : 0.0f, lq = in && drawn ? logit(p.draft + t * p.ldd, x) : 0.0f;
-        if (in) pw = weight_call(lp, sh.mp[t], p.scale_log2, sh.table) / sh.zp[t];
-        if (in && drawn) qw = weight_call(lq, sh.mq[t], p.scale_log2, sh.table) / sh.zq[t];
-        if (!drawn)                                           // a sibling's token that was rejected has nothing left
-          for (int b = t + 1; b < s; ++b)
-            if (sh.parent[b] == t && sh.token[b] == x) pw = 0.0;
+      if (in) {
+        pw = weight_call(lp, sh.mp[parent], p.scale_log2, sh.table) / sh.zp[parent];
+        if (drawn) {
+          qw = weight_call(lq, sh.mq[parent], p.scale_log2, sh.table) / sh.zq[parent];
+        } else {                                       // a sibling's token that was rejected has nothing left
+          for (int b = parent + 1; b < tid; ++b)
+            if (sh.parent[b] == parent && sh.token[b] == token) pw = 0.0;
+        }
       }
-      sh.pw[s] = pw;
-      sh.qw[s] = qw;
+      sh.pw[tid] = pw;
+      sh.qw[tid] = qw;
     }
     __syncthreads();
   }
@@ -485,6 +542,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
     double left = 1.0;                                 // point drafts: what the rejected siblings leave
     int rejected = 0, taken = -1;
     Residual r{0.0, 1.0, 0};
+    const Ahead first = fetch_rounds(p, drawn ? p.max_children : 0, t, lane);
     for (int s0 = t + 1; s0 < p.nodes && taken < 0; s0 += 64) {
       unsigned long long hits = __ballot(s0 + lane < p.nodes && sh.parent[min(s0 + lane, kNodes - 1)] == t);
       for (; hits && taken < 0; hits &= hits - 1) {
@@ -499,13 +557,18 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
         } else {
           if (rejected == p.max_children) break;
           ok = (double)sh.u[s] * sh.qw[s] * r.s < fmax(sh.pw[s] - r.a * sh.qw[s], 0.0);
-          if (!ok) reject(p, t, rejected + 1, lane, r);
+          if (!ok) reject(p, t, rejected + 1, lane, first, r);
           ++rejected;
         }
         if (ok) taken = s;
       }
     }
-    if (lane == 0) sh.next[t] = taken;
+    if (lane == 0) {
+      sh.next[t] = taken;
+      sh.a[t] = r.a;
+      sh.s[t] = r.s;
+      sh.round[t] = r.round;
+    }
   }
   __syncthreads();
 
@@ -527,12 +590,10 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
     const uint16_t* rp = p.target + node * p.ldt;
     const float mp = sh.mp[node];
     const double ip = 1.0 / sh.zp[node];
-    Residual r{0.0, 1.0, 0};
+    const Residual r{sh.a[node], sh.s[node], sh.round[node]};
     int children = 0;
     for (int s0 = node + 1; s0 < p.nodes; s0 += 64)
       children += __builtin_popcountll(__ballot(s0 + lane < p.nodes && sh.parent[min(s0 + lane, kNodes - 1)] == node));
-    if (drawn)
-      for (int k = 1; k <= min(children, p.max_children); ++k) reject(p, node, k, lane, r);
     const double a = r.round ? r.a / sh.zq[node] : 0.0;
     const uint16_t* rq = r.round ? p.draft + node * p.ldd : nullptr;
     const float mq = r.round ? sh.mq[node] : 0.0f;
@@ -623,20 +684,15 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
       bool passed = false;
       for (int c0 = 0; c0 < p.chunks && !passed; c0 += 64) {
         const double s = c0 + lane < p.chunks ? sums[c0 + lane] : 0.0;
-        double end = s;                                // inclusive scan
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-          const double y = __shfl_up(end, d);
-          if (lane >= d) end += y;
-        }
+        const double end = wave_scan(s, lane);
         const unsigned long long some = __ballot(s > 0.0), past = __ballot(s > 0.0 && before + end > goal);
         if (some) {
           const int at = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
           chunk = c0 + at;
-          chunk_before = before + __shfl(end - s, at);
+          chunk_before = before + lane_value(end - s, at);
           passed = past != 0;
         }
-        before += __shfl(end, 63);
+        before += lane_value(end, 63);
       }
       if (lane == 0) {
         sh.chunk = chunk;
@@ -653,19 +709,13 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
       double run = 0.0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) run += w[e];
-      double end = run;                                // inclusive scan over the wave, then over the waves
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const double y = __shfl_up(end, d);
-        if (lane >= d) end += y;
-      }
+      const double end = wave_scan(run, lane);         // then over the waves
       __syncthreads();                                 // sh.wave may still be read
       if (lane == 63) sh.wave[wave] = end;
       __syncthreads();
       double ahead = lane < wave ? sh.wave[lane] : 0.0;  // the waves before this one
-#pragma unroll
-      for (int d = 8; d; d >>= 1) ahead += __shfl_xor(ahead, d);
-      double cum = sh.before + __shfl(ahead, 0) + (end - run);
+      ahead = lane_value(row16_sum64(ahead), 0);
+      double cum = sh.before + ahead + (end - run);
       int hit = -1, tail = -1;                         // the thread's first past the goal, and last with weight
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -678,7 +728,8 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
       // The first hit in index order, else the last tail.  (Not by LDS atomics: over a wave's
       // lanes those run one lane at a time.)
       const unsigned long long hits = __ballot(hit >= 0), tails = __ballot(tail >= 0);
-      const int h = __shfl(hit, hits ? __builtin_ctzll(hits) : 0), tl = __shfl(tail, tails ? 63 - __builtin_clzll(tails) : 0);
+      const int h = __builtin_amdgcn_readlane(hit, hits ? __builtin_ctzll(hits) : 0);
+      const int tl = __builtin_amdgcn_readlane(tail, tails ? 63 - __builtin_clzll(tails) : 0);
       if (lane == 0) {
         sh.hit[wave] = hits ? h : -1;
         sh.tail[wave] = tails ? tl : -1;
