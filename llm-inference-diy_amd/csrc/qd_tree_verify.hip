@@ -171,9 +171,6 @@ __device__ __forceinline__ void expand8(const f16x8u& raw, const uint16_t* row, 
       x[e] = v + e < vocab ? (float)reinterpret_cast<const _Float16*>(row)[v + e] : -__builtin_inff();
   }
 }
-__device__ __forceinline__ void load8(const uint16_t* row, int v, int vocab, float (&x)[8]) {
-  expand8(fetch8(row, v, vocab), row, v, vocab, x);
-}
 
 // Their weights; 0 past the row's end.
 __device__ __forceinline__ void weights8(const float (&x)[8], int v, int vocab, const Scale& s, const unsigned long long* table,
@@ -499,8 +496,18 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
     if (p.greedy) {
       float m = -__builtin_inff();
       int at = 0x7fffffff;
-      for (int c = c0; c < p.groups; c += 16)
-        better(m, at, p.maxes[(long long)t * p.groups + c], p.args[(long long)t * p.groups + c]);
+      for (int g0 = 0; g0 < p.groups; g0 += 64) {      // four loads at once; a group may be met twice
+        float gm[4];
+        int gi[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const long long g = (long long)t * p.groups + min(g0 + 16 * i + c0, p.groups - 1);
+          gm[i] = p.maxes[g];
+          gi[i] = p.args[g];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) better(m, at, gm[i], gi[i]);
+      }
 #pragma unroll
       for (int d = 8; d; d >>= 1) better(m, at, __shfl_xor(m, d), __shfl_xor(at, d));
       if (c0 == 0) sh.best[t] = at == 0x7fffffff ? 0 : at;
@@ -537,38 +544,68 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
     __syncthreads();
   }
 
-  // Every node's children in order, a wave per node.
+  // Every node's children in order, a wave per node.  Lanes hold a block of 64 nodes (read once
+  // where there are no more), and lane i the decision on the wave's node i.
+  static_assert(kNodes == 64 * kWalkWaves, "a lane per node of a wave");
+  int block = -1, above = -1, next = -1, round = 0;
+  double u = 0.0, pw = 0.0, qw = 0.0, ra = 0.0, rs = 1.0;
   for (int t = wave; t < p.nodes; t += kWalkWaves) {
     double left = 1.0;                                 // point drafts: what the rejected siblings leave
     int rejected = 0, taken = -1;
     Residual r{0.0, 1.0, 0};
-    const Ahead first = fetch_rounds(p, drawn ? p.max_children : 0, t, lane);
-    for (int s0 = t + 1; s0 < p.nodes && taken < 0; s0 += 64) {
-      unsigned long long hits = __ballot(s0 + lane < p.nodes && sh.parent[min(s0 + lane, kNodes - 1)] == t);
-      for (; hits && taken < 0; hits &= hits - 1) {
-        const int s = s0 + __builtin_ctzll(hits);
-        bool ok;
-        if (p.greedy) {
-          ok = sh.token[s] == sh.best[t];
-        } else if (!drawn) {
-          left = fmax(left, sh.pw[s]);                 // rounding may have taken a little of the token's own share
-          ok = (double)sh.u[s] * left < sh.pw[s];
-          left -= sh.pw[s];
-        } else {
-          if (rejected == p.max_children) break;
-          ok = (double)sh.u[s] * sh.qw[s] * r.s < fmax(sh.pw[s] - r.a * sh.qw[s], 0.0);
-          if (!ok) reject(p, t, rejected + 1, lane, first, r);
-          ++rejected;
-        }
-        if (ok) taken = s;
+    Ahead first{0.0, 0.0, 0.0};
+    for (int s0 = t & ~63; s0 < p.nodes && taken < 0; s0 += 64) {
+      if (s0 != block) {
+        const int s = s0 + lane;
+        const bool there = s < p.nodes;
+        block = s0;
+        above = there ? sh.parent[s] : -1;
+        u = there ? (double)sh.u[s] : 0.0;
+        pw = there ? sh.pw[s] : 0.0;
+        qw = there ? sh.qw[s] : 0.0;
       }
+      const bool mine = above == t;
+      unsigned long long hits = __ballot(mine);
+      if (!hits) continue;
+      if (drawn) {
+        if (rejected == 0) first = fetch_rounds(p, p.max_children, t, lane);
+        for (; hits && taken < 0 && rejected < p.max_children; hits &= hits - 1) {
+          const int c = __builtin_ctzll(hits);
+          const double q = lane_value(qw, c);
+          if (lane_value(u, c) * q * r.s < fmax(lane_value(pw, c) - r.a * q, 0.0)) {
+            taken = s0 + c;
+          } else {
+            reject(p, t, rejected + 1, lane, first, r);
+            ++rejected;
+          }
+        }
+        continue;
+      }
+      bool ok;
+      if (p.greedy) {
+        ok = mine && sh.token[s0 + lane] == sh.best[t];
+      } else {
+        const double w = mine ? pw : 0.0, upto = wave_scan(w, lane);
+        // At least the token's own share: rounding may have taken a little of it.
+        ok = u * fmax(left - (upto - w), w) < w;
+        left -= lane_value(upto, 63);
+      }
+      const unsigned long long good = __ballot(ok);
+      if (good) taken = s0 + __builtin_ctzll(good);
     }
-    if (lane == 0) {
-      sh.next[t] = taken;
-      sh.a[t] = r.a;
-      sh.s[t] = r.s;
-      sh.round[t] = r.round;
+    if (lane == t / kWalkWaves) {
+      next = taken;
+      ra = r.a;
+      rs = r.s;
+      round = r.round;
     }
+  }
+  if (wave + kWalkWaves * lane < p.nodes) {
+    const int t = wave + kWalkWaves * lane;
+    sh.next[t] = next;
+    sh.a[t] = ra;
+    sh.s[t] = rs;
+    sh.round[t] = round;
   }
   __syncthreads();
 
@@ -600,8 +637,16 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
     const double* rs = r.round ? p.rounds + ((long long)(r.round - 1) * p.nodes + node) * p.chunks : nullptr;
     const bool holes = !drawn && children;             // rejected tokens of point drafts
 
-    // This thread's eight of chunk c, without the rejected tokens.
-    auto chunk_weights = [&](int c, double (&w)[8]) {
+    // This thread's two of chunk c, without the rejected tokens.
+    constexpr int kEach = kVerifyChunk / kWalkThreads;
+    auto chunk_weights = [&](int c, double (&w)[kEach]) {
+      float x[kEach], y[kEach];
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int v = min(c * kVerifyChunk + kEach * tid + e, p.vocab - 1);
+        x[e] = logit(rp, v);
+        y[e] = rq ? logit(rq, v) : 0.0f;
+      }
       if (holes) {
         __syncthreads();                               // sh.gone may still be read
         if (tid < kVerifyChunk / 32) sh.gone[tid] = 0u;
@@ -613,37 +658,11 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
         __syncthreads();
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = 0.0;
-      const int i0 = 8 * tid, v = c * kVerifyChunk + i0;
-      if (i0 >= kVerifyChunk || v >= p.vocab) return;
-      float x[8], y[8];
-      load8(rp, v, p.vocab, x);
-      if (rq) load8(rq, v, p.vocab, y);
-      if (fabsf(mp) < __builtin_inff() && fabsf(mq) < __builtin_inff()) {   // eight at once
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const double d = ((double)x[e] - (double)mp) * p.scale_log2;
-          w[e] = d > kLeast ? exp2_32nds(d, sh.table) * ip : 0.0;   // past the row's end: -inf
-        }
-        if (rq) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const double d = ((double)y[e] - (double)mq) * p.scale_log2;
-            w[e] = fmax(w[e] - (d > kLeast ? exp2_32nds(d, sh.table) * a : 0.0), 0.0);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (v + e < p.vocab) {
-            w[e] = weight_call(x[e], mp, p.scale_log2, sh.table) * ip;
-            if (rq) w[e] = fmax(w[e] - weight_call(y[e], mq, p.scale_log2, sh.table) * a, 0.0);
-          }
-      }
-      if (holes) {
-        const unsigned gone = (sh.gone[i0 >> 5] >> (i0 & 31)) & 0xffu;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = (gone >> e) & 1u ? 0.0 : w[e];
+      for (int e = 0; e < kEach; ++e) {
+        const int i = kEach * tid + e;
+        w[e] = weight_call(x[e], mp, p.scale_log2, sh.table) * ip;
+        if (rq) w[e] = fmax(w[e] - weight_call(y[e], mq, p.scale_log2, sh.table) * a, 0.0);
+        if (c * kVerifyChunk + i >= p.vocab || (holes && (sh.gone[i >> 5] >> (i & 31)) & 1u)) w[e] = 0.0;
       }
     };
 
@@ -667,9 +686,10 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
         if (sh.parent[k] != node || sh.token[k] < 0 || sh.token[k] >= p.vocab) continue;
         const int c = sh.token[k] / kVerifyChunk;
         if (sums[c] >= 0.0) continue;                  // uniform: nothing is written between the barriers
-        double w[8];
+        double w[kEach];
         chunk_weights(c, w);
-        const double s = block_sum(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])), sh);
+        static_assert(kEach == 2, "the sum of two");
+        const double s = block_sum(w[0] + w[1], sh);
         if (tid == 0) sums[c] = s;
         __syncthreads();
       }
@@ -704,11 +724,9 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
     const int chunk = sh.chunk;
     if (chunk >= 0) {                                  // else all is rejected and nothing has weight: token 0
       const double goal = (double)sample_u * sh.total;
-      double w[8];
+      double w[kEach];
       chunk_weights(chunk, w);
-      double run = 0.0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) run += w[e];
+      const double run = w[0] + w[1];
       const double end = wave_scan(run, lane);         // then over the waves
       __syncthreads();                                 // sh.wave may still be read
       if (lane == 63) sh.wave[wave] = end;
@@ -718,11 +736,11 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
       double cum = sh.before + ahead + (end - run);
       int hit = -1, tail = -1;                         // the thread's first past the goal, and last with weight
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < kEach; ++e) {
         cum += w[e];
         if (w[e] > 0.0) {
-          tail = 8 * tid + e;
-          if (cum > goal && hit < 0) hit = 8 * tid + e;
+          tail = kEach * tid + e;
+          if (cum > goal && hit < 0) hit = kEach * tid + e;
         }
       }
       // The first hit in index order, else the last tail.  (Not by LDS atomics: over a wave's
@@ -735,12 +753,11 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
         sh.tail[wave] = tails ? tl : -1;
       }
       __syncthreads();
-      int first = -1, final = 0;
-#pragma unroll
-      for (int i = kWalkWaves - 1; i >= 0; --i) first = sh.hit[i] >= 0 ? sh.hit[i] : first;
-#pragma unroll
-      for (int i = 0; i < kWalkWaves; ++i) final = sh.tail[i] >= 0 ? sh.tail[i] : final;
-      last = chunk * kVerifyChunk + (first >= 0 ? first : final);
+      const int wh = lane < kWalkWaves ? sh.hit[lane] : -1, wt = lane < kWalkWaves ? sh.tail[lane] : -1;
+      const unsigned long long whits = __ballot(wh >= 0), wtails = __ballot(wt >= 0);
+      const int at = whits ? __builtin_amdgcn_readlane(wh, __builtin_ctzll(whits))
+                     : wtails ? __builtin_amdgcn_readlane(wt, 63 - __builtin_clzll(wtails)) : 0;
+      last = chunk * kVerifyChunk + at;
     }
   }
 
