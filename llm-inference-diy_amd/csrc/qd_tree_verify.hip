@@ -195,7 +195,7 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(TreeVerifyParams
   __shared__ float sm[64];                             // [run][wave]
   __shared__ double ss[64];
   load_arguments(p);
-  const int t = blockIdx.y, side = blockIdx.z, c = blockIdx.x * p.runs, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int t = blockIdx.y, side = blockIdx.z, c = blockIdx.x * p.runs, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint16_t* row = side ? p.draft + t * p.ldd : p.target + t * p.ldt;
   const int v0 = c * kVerifyChunk + 8 * threadIdx.x;
   f16x8u raw = fetch8(row, v0, p.vocab);
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(kThreads) void verify_round_kernel(TreeVerifyParams
   __shared__ unsigned long long table[32];
   __shared__ double ss[kVerifyRuns][kWaves];
   load_arguments(p);
-  const int t = blockIdx.y, c = blockIdx.x * p.runs, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int t = blockIdx.y, c = blockIdx.x * p.runs, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint16_t* rp = p.target + t * p.ldt;
   const uint16_t* rq = p.draft + t * p.ldd;
   const Groups g = fetch_groups(p, (lane >> 4) & 1, t, lane & 15);   // target and drafter, twice
@@ -468,7 +468,7 @@ __device__ __forceinline__ double block_sum(double x, WalkShared& sh) {
 __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyParams p) {
   __shared__ WalkShared sh;
   load_arguments(p);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool drawn = !p.greedy && p.draft != nullptr;
   const float sample_u = p.greedy ? 0.0f : *p.sample_u;
   if (!p.greedy && tid < 32) sh.table[tid] = kPow32[tid];
