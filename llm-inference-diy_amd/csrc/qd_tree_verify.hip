@@ -21,8 +21,8 @@
 //
 // Measured on MI355X: 64 rows of 151936 logits 13 us (25 instructions per logit are 15 of its 25
 // thousand cycles; the loads' and LDS latency at its two ends the rest) and the one workgroup
-// 15; 27 rows of drawn drafts over 32003 logits 5, four rounds of 3.6-6.8 and 14; the greedy
-// check of 5 rows 3.7 and 4.0.
+// 11; 27 rows of drawn drafts over 32003 logits 5, four rounds of 5.5-6.7 and 10; the greedy
+// check of 5 rows 3.9 and 4.1.
 #include "qd_device.h"
 #include "qd_internal.h"
 #include "qd_tree.h"
@@ -102,8 +102,8 @@ __device__ __forceinline__ double weight(float l, const Scale& s, const unsigned
   if (l != l) l = -__builtin_inff();
   return l == s.m ? 1.0 : 0.0;
 }
-// The same as a function of its own, for the one-workgroup kernel: its time is that of fetching
-// instructions that run once, and an inlined weight is 40 of them.
+// The same as a function of its own, where few lanes have one weight each: the time there is that
+// of fetching instructions that run once, and an inlined weight is 40 of them.
 __device__ __attribute__((noinline)) double weight_call(float l, float m, double scale, const unsigned long long* table) {
   return weight(l, make_scale(m, scale), table);
 }
