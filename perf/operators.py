@@ -162,8 +162,8 @@ def _attn_inputs(case, seed):
     T, P, H, KH = case["nodes"], case["prefix"], case["heads"], case["kv_heads"]
     s = dict(parents=_tree(rs, T, case["chain"]))
     s["q"] = _normal(g, T, H * D, scale=1.5)
-    row, _ = _kv_strides(case)
-    n = max(1, P) * (KH * D if case["layout"] == "head_major" else row)
+    row, head = _kv_strides(case)
+    n = max(1, P) * KH * D if head > row else max(1, P) * row
     s["k"], s["v"] = _normal(g, n), _normal(g, n)
     s["kt"], s["vt"] = _normal(g, T, KH * D), _normal(g, T, KH * D)
     s["out"] = torch.empty(T, H * D, dtype=torch.float16, device=DEV)
