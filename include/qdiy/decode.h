@@ -239,7 +239,8 @@ size_t qd_tree_attention_workspace_bytes(const qd_ctx* ctx, int nodes, int num_h
  *     p(tokens[c]) becomes 0.  (Drafts that are given tokens, e.g. the most
  *     likely ones or copies from the prompt.)
  *   temperature > 0 and draft_logits (row t: the drafter's logits after node t,
- *     ldd apart; rows of nodes without children are not read), the children drawn
+ *     ldd apart; rows of nodes without children are not read: the buffer may end
+ *     before them, or hold something else there), the children drawn
  *     independently from q = softmax(draft row / temperature): child c stands if
  *     accept_u[c] * q(tokens[c]) < p(tokens[c]); otherwise p becomes
  *     max(p - q, 0), normalised.  Only the first max_children children of a
@@ -259,7 +260,8 @@ size_t qd_tree_attention_workspace_bytes(const qd_ctx* ctx, int nodes, int num_h
  * 2-byte aligned, ldt and ldd >= vocab.  workspace: device memory, 16-byte
  * aligned, of qd_tree_verify_workspace_bytes(nodes, vocab, max_children) bytes.
  * Outputs and workspace overlap neither each other nor anything that is read
- * (QD_EINVAL). */
+ * (QD_EINVAL; of the draft rows only row 0 is known to the host, the others are
+ * the caller's to keep apart). */
 int qd_tree_verify(const uint16_t* target_logits, long long ldt, const uint16_t* draft_logits,
                    long long ldd, const int* tokens, const int* parents, const float* accept_u,
                    const float* sample_u, float temperature, int nodes, int vocab,

@@ -226,7 +226,8 @@ int qd_tree_verify(const uint16_t* target_logits, long long ldt, const uint16_t*
     return fail(QD_EINVAL, "workspace of %zu bytes is smaller than the %zu needed", workspace_bytes, need);
   const size_t n4 = (size_t)nodes * 4;
   const Span t{target_logits, ((size_t)(nodes - 1) * ldt + vocab) * 2};
-  const Span d{drawn ? draft_logits : nullptr, drawn ? ((size_t)(nodes - 1) * ldd + vocab) * 2 : 0};
+  // Which draft rows are read only the device knows; those of leaves may be the outputs' memory.
+  const Span d{drawn ? draft_logits : nullptr, drawn && nodes > 1 ? (size_t)vocab * 2 : 0};
   const Span au{greedy ? nullptr : accept_u, n4}, su{greedy ? nullptr : sample_u, 4};
   const Span out[4] = {{workspace, need}, {path, n4}, {emitted, n4}, {count, 4}};
   for (int i = 0; i < 4; ++i) {

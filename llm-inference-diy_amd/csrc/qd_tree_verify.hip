@@ -185,7 +185,7 @@ __device__ __forceinline__ void weights8(const float (&x)[8], int v, int vocab, 
 }
 
 // (1) Sampled: blockIdx = (p.runs chunks, node, side).  The drafter's rows of nodes without
-// children have no use.  Each wave sums each run of 512 logits relative to the run's own
+// children are not read: the buffer may end before them.  Each wave sums each run of 512 logits relative to the run's own
 // largest, so that its work on one run stands behind that run's load alone; one wave puts the
 // sums on a common base at the end.
 constexpr int kWaves = kThreads / 64;
@@ -198,12 +198,12 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(TreeVerifyParams
   const int t = blockIdx.y, side = blockIdx.z, c = blockIdx.x * p.runs, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint16_t* row = side ? p.draft + t * p.ldd : p.target + t * p.ldt;
   const int v0 = c * kVerifyChunk + 8 * threadIdx.x;
-  f16x8u raw = fetch8(row, v0, p.vocab);
-  if (side) {
+  if (side) {                                          // before any load: the row need not be there
     bool child = false;
     for (int s = t + 1 + threadIdx.x; s < p.nodes; s += kThreads) child |= p.parents[s] == t;
     if (!__syncthreads_or(child)) return;
   }
+  f16x8u raw = fetch8(row, v0, p.vocab);
   if (lane < 32) table[lane] = kPow32[lane];           // every wave writes it all, and needs no barrier to read it
 #pragma unroll 1
   for (int r = 0; r < p.runs; ++r) {

@@ -681,15 +681,17 @@ def tree_verify(target_logits: torch.Tensor, tokens: torch.Tensor, parents: torc
                 sample_u: torch.Tensor | None = None, draft_logits: torch.Tensor | None = None,
                 max_children: int = 0, ldt: int | None = None, ldd: int | None = None, stream=None) -> None:
     """qd_tree_verify: which path of a drafted tree stands against the target's logits, and the
-    token after it; greedy at temperature 0, else from the given uniforms accept_u and sample_u."""
+    token after it; greedy at temperature 0, else from the given uniforms accept_u and sample_u.
+    draft_logits needs no row for the last node, which has no children."""
     ldt = vocab if ldt is None else ldt
     ldd = vocab if ldd is None else ldd
     dev = _current_device()
     i32, f32 = torch.int32, torch.float32
     ws, ws_bytes = _workspace(workspace, dev)
+    draft_numel = (nodes - 2) * ldd + vocab if nodes > 1 else 0
     _check(load().qd_tree_verify(
         _arg(target_logits, "target_logits", _F16, dev, (nodes - 1) * ldt + vocab), ldt,
-        None if draft_logits is None else _arg(draft_logits, "draft_logits", _F16, dev, (nodes - 1) * ldd + vocab), ldd,
+        None if draft_logits is None else _arg(draft_logits, "draft_logits", _F16, dev, draft_numel), ldd,
         _arg(tokens, "tokens", i32, dev, nodes), _arg(parents, "parents", i32, dev, nodes),
         None if accept_u is None else _arg(accept_u, "accept_u", f32, dev, nodes),
         None if sample_u is None else _arg(sample_u, "sample_u", f32, dev, 1), temperature, nodes, vocab,
