@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 import numpy as np
 import torch
@@ -227,6 +228,23 @@ def _arg(t: torch.Tensor, name: str, dtype: torch.dtype, dev: int, numel: int) -
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     raise ValueError(f"{name} holds {t.numel()} elements, needs {numel}")
+
+
+def _fits(pack, names: str, *values) -> None:
+    """Refuses numbers that their C types cannot hold, of which ctypes would pass on the low bits.
+    pack: of a struct.Struct with those types (0.3 us for a call's numbers together)."""
+    try:
+        pack(*values)
+    except struct.error:
+        for name, x in zip(names.split(), values):
+            bits = 63 if name.endswith("stride") or name in ("ldt", "ldd") else 31
+            if not -1 << bits <= x < 1 << bits:
+                raise OverflowError(f"{name} {x} does not fit {bits + 1} bits") from None
+        raise TypeError(f"{names} must be whole numbers") from None
+
+
+_PACK_2I, _PACK_3I = struct.Struct("2i").pack, struct.Struct("3i").pack
+_PACK_3I2Q, _PACK_3I4Q = struct.Struct("3i2q").pack, struct.Struct("3i4q").pack
 
 
 def _workspace(t: torch.Tensor, dev: int) -> tuple:
@@ -480,6 +498,8 @@ class Context:
         qkv_stride = row if qkv_stride is None else qkv_stride
         q_stride = H * HEAD_DIM if q_stride is None else q_stride
         tree_row_stride = KH * HEAD_DIM if tree_row_stride is None else tree_row_stride
+        _fits(_PACK_3I4Q, "prefix nodes num_heads qkv_stride q_stride tree_row_stride tree_head_stride", prefix, nodes,
+              H, qkv_stride, q_stride, tree_row_stride, tree_head_stride)
         span = self._span(nodes, tree_row_stride, tree_head_stride)
         dev = _current_device()
         _check(load().qd_tree_qkv_rope(
@@ -492,7 +512,9 @@ class Context:
 
     def tree_attention_workspace_bytes(self, nodes: int, num_heads: int | None = None) -> int:
         """qd_tree_attention_workspace_bytes: enough at any prefix."""
-        n = load().qd_tree_attention_workspace_bytes(self._h, nodes, self.num_heads if num_heads is None else num_heads)
+        H = self.num_heads if num_heads is None else num_heads
+        _fits(_PACK_2I, "nodes num_heads", nodes, H)
+        n = load().qd_tree_attention_workspace_bytes(self._h, nodes, H)
         if n == 0:
             _check(QD_EINVAL)
         return n
@@ -511,6 +533,8 @@ class Context:
         q_stride = row if q_stride is None else q_stride
         out_stride = row if out_stride is None else out_stride
         tree_row_stride = KH * HEAD_DIM if tree_row_stride is None else tree_row_stride
+        _fits(_PACK_3I4Q, "prefix nodes num_heads q_stride out_stride tree_row_stride tree_head_stride", prefix, nodes, H,
+              q_stride, out_stride, tree_row_stride, tree_head_stride)
         cache = self._span(min(prefix, self.max_seqlen), self.kv_row_stride, self.kv_head_stride)
         span = self._span(nodes, tree_row_stride, tree_head_stride)
         dev = _current_device()
@@ -542,6 +566,8 @@ class Context:
                 raise ValueError("k_cache and v_cache differ in size: give cache_layer_stride")
             cache_layer_stride = k_cache.numel() // layers
         tree_row_stride = self.num_heads * HEAD_DIM if tree_row_stride is None else tree_row_stride
+        _fits(_PACK_3I4Q, "prefix nodes layers tree_layer_stride tree_row_stride tree_head_stride cache_layer_stride",
+              prefix, nodes, layers, tree_layer_stride, tree_row_stride, tree_head_stride, cache_layer_stride)
         span = self._span(nodes, tree_row_stride, tree_head_stride, (layers - 1) * tree_layer_stride)
         cache = self._span(min(self.max_seqlen, prefix + nodes), self.kv_row_stride, self.kv_head_stride,
                            (layers - 1) * cache_layer_stride)
@@ -669,6 +695,7 @@ def tree_layout(parents) -> tuple:
 
 def tree_verify_workspace_bytes(nodes: int, vocab: int, max_children: int = 0) -> int:
     """qd_tree_verify_workspace_bytes: enough in any mode."""
+    _fits(_PACK_3I, "nodes vocab max_children", nodes, vocab, max_children)
     n = load().qd_tree_verify_workspace_bytes(nodes, vocab, max_children)
     if n == 0:
         raise ValueError(f"nodes {nodes}, vocab {vocab} or max_children {max_children} out of range")
@@ -685,6 +712,7 @@ def tree_verify(target_logits: torch.Tensor, tokens: torch.Tensor, parents: torc
     draft_logits needs no row for the last node, which has no children."""
     ldt = vocab if ldt is None else ldt
     ldd = vocab if ldd is None else ldd
+    _fits(_PACK_3I2Q, "nodes vocab max_children ldt ldd", nodes, vocab, max_children, ldt, ldd)
     dev = _current_device()
     i32, f32 = torch.int32, torch.float32
     ws, ws_bytes = _workspace(workspace, dev)

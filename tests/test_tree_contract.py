@@ -88,3 +88,81 @@ def test_binding_takes_draft_logits_without_the_last_row(qdiy, binding, nodes):
         with pytest.raises(ValueError, match="draft_logits holds"):
             qdiy.tree_verify(*args, draft_logits=halves(need - 1), **kw)
         assert len(binding.calls) == 1
+
+
+# ------------------------------------------------------------------ numbers that a C int cannot hold
+
+WIDE = [2 ** 32 + 5, -2 ** 32 + 5, 2 ** 31, -2 ** 31 - 1]
+
+
+@pytest.mark.parametrize("prefix", WIDE)
+def test_binding_refuses_a_prefix_past_32_bits(qdiy, binding, prefix):
+    """ctypes keeps the low 32 bits of such a number: 2^32 + 5 would run as a prefix of 5 (and
+    with a prefix of -2^32 + 5 no cache row would have been asked for)."""
+    ctx = qdiy.Context.__new__(qdiy.Context)
+    ctx.num_heads, ctx.max_seqlen, ctx.kv_row_stride, ctx.kv_head_stride, ctx._h = 1, 64, 128, 128, None
+    x, i = halves(4096), ints(4)
+    ws = torch.zeros(4096, dtype=torch.uint8)
+    with pytest.raises(OverflowError, match="prefix"):
+        ctx.tree_qkv_rope(x, None, i, x, x, x, prefix, 2)
+    with pytest.raises(OverflowError, match="prefix"):
+        ctx.tree_attention(x, x, x, x, x, torch.zeros(2, dtype=torch.int64), x, prefix, 2, ws)
+    with pytest.raises(OverflowError, match="prefix"):
+        ctx.tree_commit(x, x, x, x, i, i, prefix, 2)
+    assert not binding.calls
+    ctx.tree_qkv_rope(x, None, i, x, x, x, 5, 2)
+    assert len(binding.calls) == 1
+
+
+@pytest.mark.parametrize("n", WIDE)
+def test_binding_refuses_counts_past_32_bits(qdiy, binding, n):
+    ctx = qdiy.Context.__new__(qdiy.Context)
+    ctx.num_heads, ctx.max_seqlen, ctx.kv_row_stride, ctx.kv_head_stride, ctx._h = 1, 64, 128, 128, None
+    x, i, ws = halves(4096), ints(4), torch.zeros(4096, dtype=torch.uint8)
+    with pytest.raises(OverflowError, match="max_children"):
+        qdiy.tree_verify(x, i, i, 2, 9, ws, i, i, i, max_children=n)
+    with pytest.raises(OverflowError, match="nodes"):
+        qdiy.tree_verify(x, i, i, n, 9, ws, i, i, i)
+    with pytest.raises(OverflowError, match="vocab"):
+        qdiy.tree_verify(x, i, i, 2, n, ws, i, i, i)
+    with pytest.raises(OverflowError, match="nodes"):
+        ctx.tree_attention(x, x, x, x, x, torch.zeros(2, dtype=torch.int64), x, 5, n, ws)
+    with pytest.raises(OverflowError, match="num_heads"):
+        ctx.tree_qkv_rope(x, None, i, x, x, x, 5, 2, num_heads=n)
+    with pytest.raises((OverflowError, ValueError), match="layers"):
+        ctx.tree_commit(x, x, x, x, i, i, 5, 2, layers=n, tree_layer_stride=0, cache_layer_stride=0)
+    for call in (lambda: ctx.tree_attention_workspace_bytes(n), lambda: ctx.tree_attention_workspace_bytes(2, n),
+                 lambda: qdiy.tree_verify_workspace_bytes(n, 9), lambda: qdiy.tree_verify_workspace_bytes(2, n),
+                 lambda: qdiy.tree_verify_workspace_bytes(2, 9, n)):
+        with pytest.raises(OverflowError):
+            call()
+    assert not binding.calls
+
+
+@pytest.mark.parametrize("stride", [2 ** 63, -2 ** 63 - 1, -2 ** 64 + 1024])
+def test_binding_refuses_strides_past_64_bits(qdiy, binding, stride):
+    """(A stride below zero makes the extents small, which are checked with Python's numbers.)"""
+    ctx = qdiy.Context.__new__(qdiy.Context)
+    ctx.num_heads, ctx.max_seqlen, ctx.kv_row_stride, ctx.kv_head_stride, ctx._h = 1, 64, 128, 128, None
+    x, i, ws = halves(4096), ints(4), torch.zeros(4096, dtype=torch.uint8)
+    m = torch.zeros(2, dtype=torch.int64)
+    for kw in ("qkv_stride", "q_stride", "tree_row_stride", "tree_head_stride"):
+        with pytest.raises(OverflowError, match=kw):
+            ctx.tree_qkv_rope(x, None, i, x, x, x, 5, 2, **{kw: stride})
+    for kw in ("q_stride", "out_stride", "tree_row_stride", "tree_head_stride"):
+        with pytest.raises(OverflowError, match=kw):
+            ctx.tree_attention(x, x, x, x, x, m, x, 5, 2, ws, **{kw: stride})
+    for kw in ("tree_layer_stride", "tree_row_stride", "tree_head_stride", "cache_layer_stride"):
+        with pytest.raises(OverflowError, match=kw):
+            ctx.tree_commit(x, x, x, x, i, i, 5, 2, **{kw: stride})
+    for kw in ("ldt", "ldd"):
+        with pytest.raises(OverflowError, match=kw):
+            qdiy.tree_verify(x, i, i, 2, 9, ws, i, i, i, **{kw: stride})
+    assert not binding.calls
+
+
+def test_binding_refuses_fractions(qdiy, binding):
+    x, i, ws = halves(4096), ints(4), torch.zeros(4096, dtype=torch.uint8)
+    with pytest.raises(TypeError, match="whole numbers"):
+        qdiy.tree_verify(x, i, i, 2, 9.5, ws, i, i, i)
+    assert not binding.calls
