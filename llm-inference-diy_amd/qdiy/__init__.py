@@ -12,6 +12,7 @@ arguments.
 from __future__ import annotations
 
 import ctypes
+import operator
 import os
 import struct
 
@@ -243,7 +244,7 @@ def _fits(pack, names: str, *values) -> None:
         raise TypeError(f"{names} must be whole numbers") from None
 
 
-_PACK_2I, _PACK_3I = struct.Struct("2i").pack, struct.Struct("3i").pack
+_PACK_I, _PACK_2I, _PACK_3I = (struct.Struct(f).pack for f in ("i", "2i", "3i"))
 _PACK_3I2Q, _PACK_3I4Q = struct.Struct("3i2q").pack, struct.Struct("3i4q").pack
 
 
@@ -685,7 +686,13 @@ def tree_layout(parents) -> tuple:
     """qd_tree_layout: (mask int64 [nodes][ceil(nodes / 64)], depth int32 [nodes]) of a drafted
     tree as CPU tensors; parents[0] is negative, parents[t] < t."""
     n = len(parents)
-    par = (ctypes.c_int * max(1, n))(*map(int, parents))
+    par = (ctypes.c_int * max(1, n))()
+    for t, p in enumerate(parents):
+        p = operator.index(p)
+        _fits(_PACK_I, "parents[t]", p)
+        par[t] = p
+    # A count out of range, or parents that make no tree, are refused before the masks are made.
+    _check(load().qd_tree_layout(par, n, None, None))
     mask = torch.empty((n, (n + 63) // 64), dtype=torch.int64)
     depth = torch.empty(n, dtype=torch.int32)
     _check(load().qd_tree_layout(par, n, ctypes.cast(mask.data_ptr(), ctypes.POINTER(ctypes.c_uint64)),

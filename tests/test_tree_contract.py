@@ -166,3 +166,35 @@ def test_binding_refuses_fractions(qdiy, binding):
     with pytest.raises(TypeError, match="whole numbers"):
         qdiy.tree_verify(x, i, i, 2, 9.5, ws, i, i, i)
     assert not binding.calls
+
+
+# ------------------------------------------------------------------ layouts
+
+@pytest.mark.parametrize("parents", [[-1, 2 ** 32], [2 ** 31, 0], [-1, 0, -2 ** 32 + 1]])
+def test_layout_refuses_parents_past_32_bits(qdiy, parents):
+    with pytest.raises(OverflowError):
+        qdiy.tree_layout(parents)
+
+
+@pytest.mark.parametrize("parents", [[-1, 0.5], [-1, "0"], [-1, None]])
+def test_layout_refuses_what_is_no_whole_number(qdiy, parents):
+    with pytest.raises(TypeError):
+        qdiy.tree_layout(parents)
+
+
+def test_layout_of_too_many_nodes_allocates_nothing(qdiy, monkeypatch):
+    """The masks of 200000 nodes would take 5 GB; the count is refused before they are made."""
+    sizes = []
+    empty = torch.empty
+    monkeypatch.setattr(qdiy.torch, "empty", lambda *a, **kw: sizes.append(a) or empty(0, **kw))
+    with pytest.raises(qdiy.QdError) as e:
+        qdiy.tree_layout([-1] + [0] * 199999)
+    assert e.value.code == qdiy.QD_EINVAL and not sizes
+
+
+def test_layout_takes_arrays_and_tensors(qdiy):
+    import numpy as np
+    want = qdiy.tree_layout([-1, 0, 0, 2])
+    for p in (np.array([-1, 0, 0, 2], np.int64), torch.tensor([-1, 0, 0, 2], dtype=torch.int32), (-1, 0, 0, 2)):
+        mask, depth = qdiy.tree_layout(p)
+        assert torch.equal(mask, want[0]) and torch.equal(depth, want[1])
