@@ -48,6 +48,10 @@ namespace {
 constexpr int kKeys = 32;
 constexpr float kLazy = 8.0f;            // log2 of the largest softmax weight before a rescale
 __device__ constexpr float kNone = -__builtin_inff();
+// A split's least weight in the fold: not 0, so that an infinity that is seen stays one however far
+// its scores lie below the row's largest, and so small that no finite value counts (at most
+// 2^40 x 2^-126 beside a denominator of at least 1).
+constexpr float kLeast = 0x1p-126f;
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
@@ -504,14 +508,14 @@ __global__ __launch_bounds__(64) void tree_attention_merge_kernel(TreeAttnParams
       }
       mn = fmaxf(mn, w[j].x);
     }
-    const float keep = mn == mx ? 1.0f : __builtin_amdgcn_exp2f(mx - mn);
+    const float keep = mn == mx ? 1.0f : fmaxf(__builtin_amdgcn_exp2f(mx - mn), kLeast);
     l *= keep;
     a0 *= keep;
     a1 *= keep;
     mx = mn;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      const float a = w[j].x == mx ? 1.0f : __builtin_amdgcn_exp2f(w[j].x - mx);   // -inf: saw no row
+      const float a = w[j].x == mx ? 1.0f : fmaxf(__builtin_amdgcn_exp2f(w[j].x - mx), kLeast);   // -inf: saw no row
       l += a * w[j].y;
       a0 += a * x[j];
       a1 += a * y[j];
