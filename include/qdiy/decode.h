@@ -205,7 +205,8 @@ int qd_tree_qkv_rope(qd_ctx* ctx, const uint16_t* qkv, long long qkv_stride, con
  * of mask (ceil(nodes / 64) words a row, device memory; any mask, not only
  * qd_tree_layout's; bits past `nodes` are ignored).  A node that sees no row
  * (prefix 0, no bit) gets zeros.  What K and V hold in rows that a node does not
- * see, infinities and NaN too, does not reach its output.  fp32 accumulation on
+ * see, infinities and NaN too, does not reach its output; infinities and NaN in
+ * V rows that it sees do, however small their weight.  fp32 accumulation on
  * the matrix cores, softmax weights rounded to fp16 for the second product: not
  * reproducible on the host, but the same bits from call to call.
  * q and out rows are [num_heads][128], q_stride and out_stride elements apart.

@@ -48,10 +48,6 @@ namespace {
 constexpr int kKeys = 32;
 constexpr float kLazy = 8.0f;            // log2 of the largest softmax weight before a rescale
 __device__ constexpr float kNone = -__builtin_inff();
-// A split's least weight in the fold: not 0, so that an infinity that is seen stays one however far
-// its scores lie below the row's largest, and so small that no finite value counts (at most
-// 2^40 x 2^-126 beside a denominator of at least 1).
-constexpr float kLeast = 0x1p-126f;
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
@@ -109,6 +105,47 @@ __device__ __forceinline__ int row_node(int r, int group) {
   if (t * group > r) --t;
   if ((t + 1) * group <= r) ++t;
   return t;
+}
+
+// Outputs that are no numbers: dims 32 g + 8 i + e of query row r, for a whole wave.  The weight of
+// a seen row may have rounded to 0 (its own, or its split's), which makes NaN of an infinity in V:
+// where V holds infinities or NaN that the row sees, the output is their sum, whatever their
+// weights.  weighed: the row's weights are numbers, and not all 0.  (Runs for such rows alone: a
+// wave reads a column of the cache, 64 rows at a time.)
+__device__ __forceinline__ bool no_number(f32x4 y) {     // (sums of weighted halves are far from overflow)
+  return !(fabsf((y[0] + y[1]) + (y[2] + y[3])) < __builtin_inff());
+}
+__device__ __forceinline__ float infinity_at(const uint16_t* v) {
+  const float y = (float)*reinterpret_cast<const _Float16*>(v);
+  return fabsf(y) < __builtin_inff() ? 0.0f : y;
+}
+__device__ __forceinline__ f32x4 with_infinities(const TreeAttnParams& p, f32x4 y, int kh, int r, int e, bool weighed) {
+  const int lane = threadIdx.x & 63, g = lane >> 4;
+  const uint64_t* mask = p.mask + (long long)row_node(r, p.group) * ((p.nodes + 63) / 64);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool odd = weighed && !(fabsf(y[i]) < __builtin_inff());
+    unsigned long long todo = __ballot(odd);
+#pragma unroll 1
+    while (todo) {                                         // dim by dim: the 16 lanes of one g
+      const int of = __builtin_ctzll(todo) >> 4, d = 32 * of + 8 * i + e;
+      todo &= ~(0xffffull << (16 * of));
+      const uint16_t* v = p.v + kh * p.head_stride + d;
+      float x = 0.0f;
+#pragma unroll 4
+      for (int j = lane; j < p.prefix; j += 64) x += infinity_at(v + j * p.row_stride);
+#pragma unroll
+      for (int s = 32; s; s >>= 1) x += __shfl_xor(x, s);
+      if (odd && g == of) {
+        const uint16_t* vt = p.vt + kh * p.thead_stride + d;
+#pragma unroll 1
+        for (int j = 0; j < p.nodes; ++j)
+          if ((mask[j >> 6] >> (j & 63)) & 1u) x += infinity_at(vt + j * p.trow_stride);
+        if (x != 0.0f) y[i] = x;                           // NaN, too
+      }
+    }
+  }
+  return y;
 }
 
 template <int kQ, int kQW, int kKW>
@@ -303,7 +340,8 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
     weights(st, pb);
   };
   // A weight of 0 keeps a finite V row out of a product, but not an infinity or a NaN: in a node
-  // tile such elements count as 0, and the fold adds them where they are seen.
+  // tile, whose rows may be unseen, such elements count as 0, and the fold adds them where they are
+  // seen.  (The cache's rows are all seen: with_infinities finds what became of theirs.)
   bool nonfinite = false;
   auto make_finite = [&](auto& v) {
     constexpr int n = sizeof(v) / sizeof(u32x4);
@@ -447,6 +485,7 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
     }
   }
   if (p.splits > 1 && live && (f0 & 7) == 0 && g == 0) p.part_ml[(long long)slot * kRows + q] = float2{mx, l};
+  unsigned odd = 0;                                        // the wave's fragments with no numbers in them
 #pragma unroll
   for (int n = 0; n < kOwn; ++n) {
     const int f = f0 + n;
@@ -457,9 +496,14 @@ __global__ __launch_bounds__(kQW * kKW * 64) void tree_attention_kernel(TreeAttn
       if (live) p.part_o[((long long)slot * kFrags + f) * 64 + lane] = acc;
     } else {
       frag[f * 64 + lane] = l == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc * inv;   // read by this wave alone
+      odd |= (__any(no_number(acc)) ? 1u : 0u) << n;
     }
   }
   if (p.splits > 1) return;
+  for (; odd; odd &= odd - 1) {
+    const int f = f0 + __builtin_ctz(odd);
+    frag[f * 64 + lane] = with_infinities(p, frag[f * 64 + lane], kh, min(r0 + q, rows - 1), f & 7, l == l && l != 0.0f);
+  }
   __syncthreads();
   const float* folded = reinterpret_cast<const float*>(frag);
   for (int i = threadIdx.x; i < kRows * 16; i += kThreads) {
@@ -508,20 +552,29 @@ __global__ __launch_bounds__(64) void tree_attention_merge_kernel(TreeAttnParams
       }
       mn = fmaxf(mn, w[j].x);
     }
-    const float keep = mn == mx ? 1.0f : fmaxf(__builtin_amdgcn_exp2f(mx - mn), kLeast);
+    const float keep = mn == mx ? 1.0f : __builtin_amdgcn_exp2f(mx - mn);
     l *= keep;
     a0 *= keep;
     a1 *= keep;
     mx = mn;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      const float a = w[j].x == mx ? 1.0f : fmaxf(__builtin_amdgcn_exp2f(w[j].x - mx), kLeast);   // -inf: saw no row
+      const float a = w[j].x == mx ? 1.0f : __builtin_amdgcn_exp2f(w[j].x - mx);   // -inf: saw no row
       l += a * w[j].y;
       a0 += a * x[j];
       a1 += a * y[j];
     }
   }
-  if (r >= p.nodes * group) return;
+  const bool live = r < p.nodes * group;
+  if (__any(live && no_number(a0 + a1))) {
+#pragma unroll 1
+    for (int k = 0; k < 2; ++k) {                          // a0, then a1
+      const f32x4 y = with_infinities(p, a0, kh, min(r, p.nodes * group - 1), 2 * pair + k, live && l == l && l != 0.0f);
+      a0 = a1;
+      a1 = y;
+    }
+  }
+  if (!live) return;
   const int t = row_node(r, group);
   const float inv = 1.0f / l;
   _Float16* out = reinterpret_cast<_Float16*>(p.out) + t * p.out_stride + (kh * group + (r - t * group)) * 128 + 32 * g + 2 * pair;

@@ -90,3 +90,64 @@ def test_a_nodes_infinity_reaches_those_that_see_it(qdiy, H, KH, P, T, gap):
     for d in (5, 77, 126):
         a[see, :, d] = b[see, :, d] = 0
     assert np.array_equal(a.view(np.uint16), b.view(np.uint16))
+
+
+@pytest.mark.parametrize("H,KH,P,T", [(2, 2, 40, 5), (2, 2, 2000, 20), (1, 1, 9000, 3), (2, 1, 3000, 24),
+                                      (2, 2, 5000, 100), (2, 2, 9, 64), (16, 16, 1203, 70)])
+@pytest.mark.parametrize("gap", [False, True])
+def test_a_cached_infinity_reaches_every_node(qdiy, H, KH, P, T, gap):
+    """Cache rows are seen by all, however small their weight: infinities and NaN reach their
+    column of every output, and no other column changes."""
+    c = Attention(qdiy, H, KH, P, T, seed=P + T, kscale=0.2)
+    if gap:
+        far_below(c)
+    c.upload()
+    a = c.result().copy()
+    assert np.all(np.isfinite(a))
+    far = [1, P // 3, P // 2, P - 2, P - 1]
+    for i, (j, bad) in enumerate(zip(far, (np.inf, -np.inf, np.nan, np.inf, -np.inf))):
+        c.V[j, :, 20 + 25 * i] = bad
+    c.V[1, :, 0] = np.inf
+    c.V[P - 1, :, 0] = -np.inf
+    c.upload()
+    b = c.result().copy()
+    for i, bad in enumerate((np.inf, -np.inf, np.nan, np.inf, -np.inf)):
+        assert np.array_equal(b[:, :, 20 + 25 * i], np.full((T, H), bad, np.float16), equal_nan=True)
+    assert np.all(np.isnan(b[:, :, 0]))                      # inf - inf
+    for d in (0, 20, 45, 70, 95, 120):
+        a[:, :, d] = b[:, :, d] = 0
+    assert np.array_equal(a.view(np.uint16), b.view(np.uint16))
+
+
+def test_infinities_in_the_cache_and_in_nodes(qdiy):
+    """Those of the cache reach all nodes, a node's those that see it."""
+    T = 30
+    vis = ancestors(chain_parents(T))
+    vis[:, 4] = False
+    vis[9, 4] = True
+    c = Attention(qdiy, 2, 2, 700, T, seed=3, vis=vis, kscale=0.2)
+    a = c.result().copy()
+    c.V[333, :, 8] = np.inf
+    c.Vt[4, :, 9] = np.inf
+    c.Vt[4, 0, 8] = -np.inf
+    c.Kt[4] = np.nan                                         # unseen but by node 9, which sees its NaN score
+    c.upload()
+    b = c.result().copy()
+    others = [t for t in range(T) if t != 9]
+    assert np.all(b[others][:, :, 8] == np.inf) and np.all(np.isnan(b[9]))
+    a[9] = b[9] = 0
+    a[:, :, 8] = b[:, :, 8] = 0
+    assert np.array_equal(a.view(np.uint16), b.view(np.uint16))
+
+
+def test_scores_that_are_no_numbers_stay_with_their_row(qdiy):
+    """A NaN in one node's q leaves the other nodes' bits as they are."""
+    for P, T in ((50, 7), (3000, 40), (3000, 130)):
+        c = Attention(qdiy, 2, 2, P, T, seed=P)
+        a = c.result().copy()
+        c.q[3, 1, 17] = np.nan
+        c.gq = dev(c.q.reshape(T, -1))
+        b = c.result().copy()
+        assert np.all(np.isnan(b[3, 1]))
+        a[3, 1] = b[3, 1] = 0
+        assert np.array_equal(a.view(np.uint16), b.view(np.uint16))
