@@ -193,7 +193,9 @@ int qd_tree_layout(const int* parents, int nodes, uint64_t* mask, int* depth);
  * outside [0, max_seqlen) gets NaN in all three rows, so that the mistake shows.
  * All fp16 buffers 16-byte aligned, strides multiples of 8; depth 4-byte
  * aligned; k_tree, v_tree and q_out must not overlap the inputs otherwise, nor
- * q_out the node rows (QD_EINVAL). */
+ * q_out the node rows, nor K and V rows each other or themselves: of rows, heads
+ * and the step from k_tree to v_tree each is at least what those of smaller steps
+ * reach (QD_EINVAL). */
 int qd_tree_qkv_rope(qd_ctx* ctx, const uint16_t* qkv, long long qkv_stride, const uint16_t* bias,
                      const int* depth, uint16_t* q_out, long long q_stride, uint16_t* k_tree,
                      uint16_t* v_tree, long long tree_row_stride, long long tree_head_stride,
@@ -281,7 +283,8 @@ size_t qd_tree_verify_workspace_bytes(int nodes, int vocab, int max_children);
  * were.  The node rows may be the cache's own rows from prefix on, in every layer
  * (k_tree == k_cache + prefix*kv_row_stride, v alike, all strides the caches'),
  * with path ascending: the path's rows are then moved up in place.  Otherwise
- * they must not overlap the caches (QD_EINVAL).  fp16 pointers 16-byte aligned,
+ * they must not overlap the caches, nor the caches' rows each other (as in
+ * qd_tree_qkv_rope; with layers) (QD_EINVAL).  fp16 pointers 16-byte aligned,
  * strides multiples of 8. */
 int qd_tree_commit(qd_ctx* ctx, const uint16_t* k_tree, const uint16_t* v_tree,
                    long long tree_layer_stride, long long tree_row_stride,

@@ -1,5 +1,6 @@
 // C ABI of the drafted-token trees: argument checks, workspaces and launches.
 // Declared in include/qdiy/decode.h.
+#include <algorithm>
 #include <cmath>
 #include <initializer_list>
 
@@ -57,6 +58,26 @@ size_t row_span(long long rows, long long row_stride, int heads, long long head_
   if (rows < 1) return 0;
   return ((size_t)(rows - 1) * row_stride + (size_t)(heads - 1) * head_stride + QD_HEAD_DIM) * 2;
 }
+
+// Whether rows of 128 halves that are written at these strides keep apart: every dimension steps
+// past what the dimensions of smaller strides reach.  (All layouts that nest do; others are
+// refused, also where their rows happen to miss each other.)
+struct Dim {
+  long long n, stride;
+};
+template <int kDims>
+bool rows_apart(Dim (&d)[kDims]) {
+  std::sort(d, d + kDims, [](const Dim& a, const Dim& b) { return a.stride < b.stride; });
+  long long reach = QD_HEAD_DIM;
+  for (const Dim& x : d) {
+    if (x.n < 2) continue;
+    if (x.stride < reach) return false;
+    reach += (x.n - 1) * x.stride;
+  }
+  return true;
+}
+// K and V rows of the same strides are two of a kind, this far apart.
+Dim k_and_v(const uint16_t* k, const uint16_t* v) { return {2, (long long)(k < v ? v - k : k - v)}; }
 
 struct Span {
   const void* p;
@@ -122,6 +143,8 @@ int qd_tree_qkv_rope(qd_ctx* ctx, const uint16_t* qkv, long long qkv_stride, con
   const Span k{k_tree, span}, v{v_tree, span};
   if (any_overlap(k, {in, b, d, q}) || any_overlap(v, {in, b, d, q}))
     return fail(QD_EINVAL, "k_tree or v_tree overlaps qkv, bias, depth or q_out");
+  Dim dims[3] = {{nodes, tree_row_stride}, {kvh, tree_head_stride}, k_and_v(k_tree, v_tree)};
+  if (!rows_apart(dims)) return fail(QD_EINVAL, "k_tree's and v_tree's rows overlap each other or themselves");
   const bool in_place = q_out == qkv && q_stride == qkv_stride;
   if (any_overlap(q, {b, d}) || (!in_place && overlaps(q.p, q.n, in.p, in.n)))
     return fail(QD_EINVAL, "q_out overlaps bias, depth or (other than in place) qkv");
@@ -297,6 +320,11 @@ int qd_tree_commit(qd_ctx* ctx, const uint16_t* k_tree, const uint16_t* v_tree, 
   const long long at = (long long)prefix * c.kv_row_stride;
   const bool in_place = k_tree == k_cache + at && v_tree == v_cache + at && tree_row_stride == c.kv_row_stride &&
                         tree_head_stride == c.kv_head_stride && (layers == 1 || tree_layer_stride == cache_layer_stride);
+  Dim dims[4] = {{std::min(nodes, c.max_seqlen - prefix), c.kv_row_stride},
+                 {kvh, c.kv_head_stride},
+                 {layers, cache_layer_stride},
+                 k_and_v(k_cache, v_cache)};
+  if (!rows_apart(dims)) return fail(QD_EINVAL, "the caches' rows overlap each other or themselves");
   const Span kc{k_cache, cache}, vc{v_cache, cache};
   if (any_overlap(kc, {{path, (size_t)nodes * 4}, {count, 4}}) || any_overlap(vc, {{path, (size_t)nodes * 4}, {count, 4}}))
     return fail(QD_EINVAL, "path or count overlaps the caches");

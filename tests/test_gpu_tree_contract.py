@@ -151,3 +151,62 @@ def test_scores_that_are_no_numbers_stay_with_their_row(qdiy):
         assert np.all(np.isnan(b[3, 1]))
         a[3, 1] = b[3, 1] = 0
         assert np.array_equal(a.view(np.uint16), b.view(np.uint16))
+
+
+# ------------------------------------------------------------------ what outputs may overlap
+
+def test_rope_refuses_node_rows_over_each_other(qdiy):
+    """K rows over V rows, rows over rows and heads over heads would race; rows that only share
+    their buffer are taken."""
+    H, KH, T = 4, 2, 3
+    ctx = qdiy.Context(num_heads=KH, max_seqlen=50)
+    W = (H + 2 * KH) * 128
+    x = dev(np.random.default_rng(1).standard_normal((T, W)).astype(np.float16))
+    depth, q = torch.zeros(T, dtype=torch.int32, device="cuda"), torch.zeros(T, H * 128, dtype=torch.float16, device="cuda")
+    want = [torch.zeros(T, KH, 128, dtype=torch.float16, device="cuda") for _ in range(2)]
+    ctx.tree_qkv_rope(x, None, depth, q, *want, 5, T, num_heads=H)
+    buf = torch.zeros(1 << 14, dtype=torch.float16, device="cuda")
+    row = KH * 128
+
+    def call(at, trow, thead):
+        ctx.tree_qkv_rope(x, None, depth, q, buf, buf[at:], 5, T, num_heads=H, tree_row_stride=trow,
+                          tree_head_stride=thead)
+
+    for at, trow, thead in ((0, row, 128), (128, row, 128), (row, row, 128), (2 * row, row, 128), (64, 2 * row, 256),
+                            (8192, 8, 128), (8192, row - 8, 128), (8192, row, 120), (8192, row, 8),
+                            (8192, 128, 3 * 128 - 8), (8192, 128, 128), (row, 2 * row - 8, 128)):
+        with pytest.raises(qdiy.QdError) as e:
+            call(at, trow, thead)
+        assert e.value.code == qdiy.QD_EINVAL, (at, trow, thead)
+    for at, trow, thead in ((row, 2 * row, 128), (128, 2 * row, 256), (8192, row, 128), (8192, 128, 3 * 128),
+                            (3 * row, row, 128), (3 * 128, 128, 6 * 128), (KH * 128 + 64, 3 * row, 128)):
+        buf.zero_()
+        call(at, trow, thead)
+        for w, base in zip(want, (0, at)):
+            got = torch.as_strided(buf, (T, KH, 128), (trow, thead, 1), base)
+            assert torch.equal(got, w), (at, trow, thead)
+
+
+def test_commit_refuses_cache_rows_over_each_other(qdiy):
+    H, L, S, T, P = 2, 3, 40, 5, 10
+    ctx = qdiy.Context(num_heads=H, max_seqlen=S)
+    row = H * 128
+    rng = np.random.default_rng(2)
+    kt, vt = (dev(rng.standard_normal((L, T, row)).astype(np.float16)) for _ in range(2))
+    path, count = dev(np.array([0, 2, 3, -1, -1], np.int32)), dev(np.array([3], np.int32))
+    buf = torch.zeros(4 * L * S * row, dtype=torch.float16, device="cuda")
+
+    def call(at, layer):
+        ctx.tree_commit(kt, vt, buf, buf[at:], path, count, P, T, layers=L, cache_layer_stride=layer)
+
+    for at, layer in ((0, S * row), (row, S * row), (128, S * row), (L * S * row, 8), (L * S * row, row),
+                      (L * S * row, (T - 1) * row), (S * row, S * row)):
+        with pytest.raises(qdiy.QdError) as e:
+            call(at, layer)
+        assert e.value.code == qdiy.QD_EINVAL, (at, layer)
+    for at, layer in ((L * S * row, S * row), (S * row, 2 * S * row), (3 * S * row, S * row)):
+        buf.zero_()
+        call(at, layer)
+        for t, base in ((kt, 0), (vt, at)):
+            got = torch.as_strided(buf, (L, S, row), (layer, row, 1), base)
+            assert torch.equal(got[:, P:P + 3], t[:, [0, 2, 3]])
