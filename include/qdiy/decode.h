@@ -280,7 +280,7 @@ size_t qd_tree_verify_workspace_bytes(int nodes, int vocab, int max_children);
  * at k_cache + l*cache_layer_stride (elements; v alike).  path and count are
  * device memory (qd_tree_verify's); entries outside [0, nodes), rows at or past
  * max_seqlen and entries from `nodes` on are skipped; other rows are left as they
- * were.  The node rows may be the cache's own rows from prefix on, in every layer
+ * were (a cache need not reach past row prefix + nodes).  The node rows may be the cache's own rows from prefix on, in every layer
  * (k_tree == k_cache + prefix*kv_row_stride, v alike, all strides the caches'),
  * with path ascending: the path's rows are then moved up in place.  Otherwise
  * they must not overlap the caches, nor the caches' rows each other (as in

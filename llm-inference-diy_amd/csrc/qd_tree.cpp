@@ -316,7 +316,7 @@ int qd_tree_commit(qd_ctx* ctx, const uint16_t* k_tree, const uint16_t* v_tree, 
   const qd_cfg& c = ctx->cfg;
   const int kvh = c.num_heads;
   const size_t tree = (size_t)(layers - 1) * tree_layer_stride * 2 + row_span(nodes, tree_row_stride, kvh, tree_head_stride);
-  const size_t cache = (size_t)(layers - 1) * cache_layer_stride * 2 + row_span(c.max_seqlen, c.kv_row_stride, kvh, c.kv_head_stride);
+  const size_t cache = (size_t)(layers - 1) * cache_layer_stride * 2 + row_span(std::min(prefix + nodes, c.max_seqlen), c.kv_row_stride, kvh, c.kv_head_stride);
   const long long at = (long long)prefix * c.kv_row_stride;
   const bool in_place = k_tree == k_cache + at && v_tree == v_cache + at && tree_row_stride == c.kv_row_stride &&
                         tree_head_stride == c.kv_head_stride && (layers == 1 || tree_layer_stride == cache_layer_stride);

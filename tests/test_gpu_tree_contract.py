@@ -210,3 +210,31 @@ def test_commit_refuses_cache_rows_over_each_other(qdiy):
         for t, base in ((kt, 0), (vt, at)):
             got = torch.as_strided(buf, (L, S, row), (layer, row, 1), base)
             assert torch.equal(got[:, P:P + 3], t[:, [0, 2, 3]])
+
+
+def test_commit_takes_a_cache_that_ends_with_its_rows(qdiy):
+    """A cache shorter than the context's max_seqlen, which holds every row that the call can
+    write: what lies behind it in the same buffer is not the cache."""
+    H, L, S, T, P = 2, 2, 400, 5, 10
+    ctx = qdiy.Context(num_heads=H, max_seqlen=S)
+    row, rows = H * 128, P + T
+    rng = np.random.default_rng(4)
+    n, m = L * rows * row, L * T * row
+    buf = torch.zeros(2 * n + 2 * m + 64, dtype=torch.float16, device="cuda")
+    kc, vc, kt, vt = buf[:n], buf[n:2 * n], buf[2 * n:2 * n + m], buf[2 * n + m:2 * n + 2 * m]
+    path, count = buf[2 * n + 2 * m:][:2 * T].view(torch.int32), buf[2 * n + 2 * m + 32:][:2].view(torch.int32)
+    x = dev(rng.standard_normal(2 * m).astype(np.float16))
+    buf[2 * n:2 * n + 2 * m].copy_(x)
+    path.copy_(dev(np.array([0, 1, 4, -1, -1], np.int32)))
+    count.fill_(3)
+    ctx.tree_commit(kt, vt, kc, vc, path, count, P, T, layers=L)
+    for c, t in ((kc, x[:m]), (vc, x[m:])):
+        got, want = c.view(L, rows, row), t.view(L, T, row)
+        assert torch.equal(got[:, P:P + 3], want[:, [0, 1, 4]])
+        assert not got[:, :P].any() and not got[:, P + 3:].any()
+    assert torch.equal(buf[2 * n:2 * n + 2 * m], x)
+    for bad in (dict(path=kc[:2 * T].view(torch.int32)), dict(count=vc[n - 8:].view(torch.int32)), dict(k_tree=vc)):
+        a = dict(k_tree=kt, v_tree=vt, k_cache=kc, v_cache=vc, path=path, count=count)
+        a.update(bad)
+        with pytest.raises(qdiy.QdError):
+            ctx.tree_commit(**a, prefix=P, nodes=T, layers=L, tree_layer_stride=T * row)
