@@ -8,7 +8,8 @@ import torch
 
 from test_gpu_tree_attention import Case as Attention
 from test_gpu_tree_verify import Case as Verify, dev
-from tree_common import ancestors, chain_parents
+from tree_common import ancestors, attention, chain_parents
+from tree_plan import attention_plan
 
 pytestmark = pytest.mark.gpu
 
@@ -238,3 +239,35 @@ def test_commit_takes_a_cache_that_ends_with_its_rows(qdiy):
         a.update(bad)
         with pytest.raises(qdiy.QdError):
             ctx.tree_commit(**a, prefix=P, nodes=T, layers=L, tree_layer_stride=T * row)
+
+
+# ------------------------------------------------------------------ attention: long scans in several splits
+
+# H, KH, P, T, then the blocks' rows, splits and rounds that they are there for (256 CUs): several
+# splits of three rounds and more, odd and even, so that LDS buffers are written again while others
+# still read, tiles loaded ahead are used, and a split's tiles lie a hop apart.
+LONG = [(64, 64, 3001, 5, 16, 4, 3), (64, 64, 3999, 13, 16, 4, 4), (16, 4, 50000, 3, 16, 49, 4), (64, 32, 9001, 8, 16, 8, 5),
+        (64, 64, 3001, 27, 32, 4, 3), (64, 32, 8101, 15, 32, 8, 4), (2, 1, 99990, 11, 32, 196, 2),
+        (128, 128, 701, 40, 64, 2, 3), (64, 64, 1917, 64, 64, 4, 4), (64, 16, 3331, 12, 64, 14, 2), (32, 8, 6100, 48, 64, 10, 5),
+        (64, 64, 601, 128, 128, 4, 3), (64, 64, 701, 100, 128, 4, 4), (32, 8, 4801, 64, 128, 16, 5), (16, 16, 4001, 250, 128, 8, 9)]
+
+
+@pytest.mark.parametrize("H,KH,P,T,block,splits,rounds", LONG)
+def test_long_scans_in_several_splits(qdiy, H, KH, P, T, block, splits, rounds):
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    plan = attention_plan(T, H, KH, P, cus)
+    if cus == 256:
+        assert (plan[0], plan[3], plan[4]) == (block, splits, rounds)
+    c = Attention(qdiy, H, KH, P, T, seed=P)
+    assert c.ws.numel() == plan[2] * KH * plan[5] * plan[0] * 130 * 4
+    a = c.result().copy()
+    assert np.all(np.isfinite(a))
+    G = H // KH
+    for kh in sorted({0, KH // 2, KH - 1}):                  # a float64 sample of the heads, all nodes
+        hs = slice(kh * G, kh * G + G)
+        want, bound = attention(c.q[:, hs], c.K[:, kh:kh + 1], c.V[:, kh:kh + 1], c.Kt[:, kh:kh + 1], c.Vt[:, kh:kh + 1],
+                                c.vis, with_bound=True)
+        err = np.abs(a[:, hs].astype(np.float64) - want)
+        assert np.all(err <= bound), np.max(err / bound)
+    for _ in range(4):                                       # a race would show in some call's bits
+        assert np.array_equal(a.view(np.uint16), c.result().view(np.uint16))

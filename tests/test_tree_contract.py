@@ -2,9 +2,12 @@
 count as read or written, and what the Python binding lets through to the C call."""
 import ctypes
 import os
+import subprocess
 
 import pytest
 import torch
+
+from conftest import ROOT
 
 
 @pytest.fixture(scope="module")
@@ -198,3 +201,28 @@ def test_layout_takes_arrays_and_tensors(qdiy):
     for p in (np.array([-1, 0, 0, 2], np.int64), torch.tensor([-1, 0, 0, 2], dtype=torch.int32), (-1, 0, 0, 2)):
         mask, depth = qdiy.tree_layout(p)
         assert torch.equal(mask, want[0]) and torch.equal(depth, want[1])
+
+
+# ------------------------------------------------------------------ attention's plan
+
+def test_the_restated_plan_is_the_librarys(tmp_path):
+    """tests/tree_plan.py chooses the GPU tests' sizes by block, splits and rounds."""
+    from tree_plan import attention_plan
+    src, lib = tmp_path / "shim.cpp", tmp_path / "shim.so"
+    src.write_text("""
+#include "qd_tree.h"
+extern "C" void plan(int nodes, int heads, int kv_heads, int prefix, int cus, int* out) {
+  const qd::TreeAttnPlan p = qd::tree_attn_plan(nodes, heads, kv_heads, prefix, cus, out + 5);
+  out[0] = p.block_rows, out[1] = p.key_waves, out[2] = p.blocks, out[3] = p.splits, out[4] = p.rounds;
+}
+""")
+    csrc = os.path.join(ROOT, "llm-inference-diy_amd", "csrc")
+    subprocess.run(["hipcc", "-x", "c++", "-D__HIP_PLATFORM_AMD__", "-std=c++17", "-shared", "-fPIC", "-I", csrc, "-I",
+                    "/opt/rocm/include", "-o", str(lib), str(src)], check=True)
+    plan = ctypes.CDLL(str(lib)).plan
+    out = (ctypes.c_int * 6)()
+    for nodes in (1, 5, 16, 17, 32, 33, 64, 65, 100, 128, 129, 250, 1024):
+        for heads, kv_heads in ((1, 1), (16, 16), (32, 8), (28, 4), (71, 1), (64, 64), (300, 300)):
+            for prefix in (0, 1, 32, 33, 512, 700, 2000, 8191, 32700):
+                plan(nodes, heads, kv_heads, prefix, 256, out)
+                assert tuple(out) == attention_plan(nodes, heads, kv_heads, prefix, 256), (nodes, heads, kv_heads, prefix)
