@@ -247,7 +247,8 @@ size_t qd_tree_attention_workspace_bytes(const qd_ctx* ctx, int nodes, int num_h
  *     independently from q = softmax(draft row / temperature): child c stands if
  *     accept_u[c] * q(tokens[c]) < p(tokens[c]); otherwise p becomes
  *     max(p - q, 0), normalised.  Only the first max_children children of a
- *     node are tested (1 <= max_children <= 64; not read in the other modes).
+ *     node are tested (1 <= max_children <= 64; not read in the other modes,
+ *     nor for one node).
  *   The last token of the two sampled modes is the first index whose cumulative
  *   p exceeds sample_u[0] times its total.
  * In both sampled modes the emitted tokens are distributed as the target's when
@@ -261,7 +262,8 @@ size_t qd_tree_attention_workspace_bytes(const qd_ctx* ctx, int nodes, int num_h
  *   count[0]:       the number of entries of both (1 + accepted drafts)
  * tokens, parents, u and the outputs are device memory, 4-byte aligned; logits
  * 2-byte aligned, ldt and ldd >= vocab.  workspace: device memory, 16-byte
- * aligned, of qd_tree_verify_workspace_bytes(nodes, vocab, max_children) bytes.
+ * aligned, of qd_tree_verify_workspace_bytes(nodes, vocab, max_children) bytes
+ * (enough with a max_children of 0 where it is not read).
  * Outputs and workspace overlap neither each other nor anything that is read
  * (QD_EINVAL; of the draft rows only row 0 is known to the host, the others are
  * the caller's to keep apart). */

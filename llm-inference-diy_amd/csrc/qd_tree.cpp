@@ -230,7 +230,8 @@ int qd_tree_verify(const uint16_t* target_logits, long long ldt, const uint16_t*
   if (temperature > 0.0f && temperature < 1e-6f)
     return fail(QD_EINVAL, "temperature %g is below 1e-6 (0 is greedy)", (double)temperature);
   const bool greedy = temperature == 0.0f, drawn = !greedy && draft_logits;
-  if (max_children < 0 || max_children > 64 || (drawn && nodes > 1 && max_children < 1))
+  const int most = drawn && nodes > 1 ? max_children : 0;   // rounds of rejected siblings
+  if (drawn && nodes > 1 && (most < 1 || most > 64))
     return fail(QD_EINVAL, "max_children %d outside [1, 64]", max_children);
   if (!target_logits || !tokens || !parents || !path || !emitted || !count || !workspace)
     return fail(QD_EINVAL, "target_logits, tokens, parents, path, emitted, count and workspace must be non-NULL");
@@ -244,7 +245,7 @@ int qd_tree_verify(const uint16_t* target_logits, long long ldt, const uint16_t*
   if (!aligned16(workspace)) return fail(QD_EINVAL, "workspace must be 16-byte aligned");
   if (ldt < vocab || ldt > kMaxStride || (drawn && (ldd < vocab || ldd > kMaxStride)))
     return fail(QD_EINVAL, "ldt and ldd must be at least vocab %d", vocab);
-  const size_t need = qd_tree_verify_workspace_bytes(nodes, vocab, max_children);
+  const size_t need = qd_tree_verify_workspace_bytes(nodes, vocab, most);
   if (workspace_bytes < need)
     return fail(QD_EINVAL, "workspace of %zu bytes is smaller than the %zu needed", workspace_bytes, need);
   const size_t n4 = (size_t)nodes * 4;
@@ -278,7 +279,7 @@ int qd_tree_verify(const uint16_t* target_logits, long long ldt, const uint16_t*
   p.chunks = (vocab + qd::kVerifyChunk - 1) / qd::kVerifyChunk;
   p.runs = qd::verify_runs(nodes, p.chunks);
   p.groups = (p.chunks + p.runs - 1) / p.runs;
-  p.max_children = nodes > 1 ? max_children : 0;
+  p.max_children = most;
   p.greedy = greedy;
   const size_t rows = (size_t)nodes * p.chunks, groups = (size_t)nodes * p.groups;
   char* ws = static_cast<char*>(workspace);
@@ -289,7 +290,7 @@ int qd_tree_verify(const uint16_t* target_logits, long long ldt, const uint16_t*
   };
   p.sums = reinterpret_cast<double*>(take(2 * rows * sizeof(double)));
   p.group_sums = reinterpret_cast<double*>(take(2 * groups * sizeof(double)));
-  p.rounds = reinterpret_cast<double*>(take((size_t)max_children * rows * sizeof(double)));
+  p.rounds = reinterpret_cast<double*>(take((size_t)most * rows * sizeof(double)));
   p.maxes = reinterpret_cast<float*>(take(2 * groups * sizeof(float)));
   p.args = reinterpret_cast<int*>(take(groups * sizeof(int)));
   const hipError_t e = qd::launch_tree_verify(p, stream);

@@ -226,3 +226,22 @@ extern "C" void plan(int nodes, int heads, int kv_heads, int prefix, int cus, in
             for prefix in (0, 1, 32, 33, 512, 700, 2000, 8191, 32700):
                 plan(nodes, heads, kv_heads, prefix, 256, out)
                 assert tuple(out) == attention_plan(nodes, heads, kv_heads, prefix, 256), (nodes, heads, kv_heads, prefix)
+
+
+# ------------------------------------------------------------------ max_children
+
+@pytest.mark.parametrize("max_children", [-1, 0, 65, 1000])
+@pytest.mark.parametrize("mode", ["greedy", "point", "drawn, one node"])
+def test_max_children_is_not_read_without_drawn_siblings(qdiy, mode, max_children):
+    """Refused for path over count, which is looked at after max_children and the workspace's size."""
+    lib = qdiy.load()
+    nodes, vocab = 1 if mode.startswith("drawn") else 4, 100
+    buf = ctypes.create_string_buffer(1 << 17)
+    at = (ctypes.addressof(buf) + 255) & ~255
+    V = ctypes.c_void_p
+    p = lambda i: V(at + 8192 + 64 * i)
+    wsb = lib.qd_tree_verify_workspace_bytes(nodes, vocab, 0)
+    draft = V(at + 4096) if mode.startswith("drawn") else None
+    rc = lib.qd_tree_verify(V(at), vocab, draft, vocab, p(0), p(1), p(2), p(3), 0.0 if mode == "greedy" else 0.5, nodes,
+                            vocab, max_children, V(at + 16384), wsb, p(4), p(5), p(4), None)
+    assert rc == qdiy.QD_EINVAL and b"must not overlap" in lib.qd_last_error()
