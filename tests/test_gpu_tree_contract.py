@@ -8,7 +8,7 @@ import torch
 
 from test_gpu_tree_attention import Case as Attention
 from test_gpu_tree_verify import Case as Verify, dev
-from tree_common import ancestors, attention, chain_parents
+from tree_common import ancestors, attention, chain_parents, verify
 from tree_plan import attention_plan
 
 pytestmark = pytest.mark.gpu
@@ -271,3 +271,103 @@ def test_long_scans_in_several_splits(qdiy, H, KH, P, T, block, splits, rounds):
         assert np.all(err <= bound), np.max(err / bound)
     for _ in range(4):                                       # a race would show in some call's bits
         assert np.array_equal(a.view(np.uint16), c.result().view(np.uint16))
+
+
+# ------------------------------------------------------------------ host tensors
+
+def test_host_tensors_are_refused_by_every_call(qdiy):
+    """One argument after the other on the host; nothing is launched."""
+    ctx = qdiy.Context(num_heads=1, max_seqlen=64)
+    h, i, f = (torch.zeros(4096, dtype=t, device="cuda") for t in (torch.float16, torch.int32, torch.float32))
+    m, ws = torch.zeros(4, dtype=torch.int64, device="cuda"), torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
+    calls = [(ctx.tree_qkv_rope, dict(qkv=h, bias=h, depth=i, q_out=h, k_tree=h, v_tree=h, prefix=3, nodes=2)),
+             (ctx.tree_attention, dict(q=h, k_layer=h, v_layer=h, k_tree=h, v_tree=h, mask=m, out=h, prefix=3, nodes=2,
+                                       workspace=ws)),
+             (ctx.tree_commit, dict(k_tree=h, v_tree=h, k_cache=h, v_cache=h, path=i, count=i, prefix=3, nodes=2)),
+             (qdiy.tree_verify, dict(target_logits=h, tokens=i, parents=i, nodes=2, vocab=9, workspace=ws, path=i,
+                                     emitted=i, count=i, temperature=1.0, accept_u=f, sample_u=f, draft_logits=h,
+                                     max_children=1))]
+    n = 0
+    for call, args in calls:
+        for name, x in args.items():
+            if isinstance(x, torch.Tensor):
+                with pytest.raises(ValueError, match=f"{name} is on cpu"):
+                    call(**dict(args, **{name: x.cpu()}))
+                n += 1
+    assert n == 6 + 8 + 6 + 10
+
+
+# ------------------------------------------------------------------ a captured step
+
+def test_a_captured_step_holds_for_its_prefix(qdiy):
+    """A step of two layers captured at one prefix and replayed with other activations, drafts,
+    random numbers and caches of that length, with eager work between: every replay gives the
+    eager step's bits.  (Prefix is the host's number: a step at another prefix is another graph.)"""
+    H, L, V, T, S, P = 4, 2, 611, 23, 160, 70
+    row = H * 128
+    rng = np.random.default_rng(23)
+    ctx = qdiy.Context(num_heads=H, max_seqlen=S)
+    half = lambda *n: torch.empty(*n, dtype=torch.float16, device="cuda")
+    kc, vc, kt, vt = half(L, S, row), half(L, S, row), half(L, T, row), half(L, T, row)
+    qkv, q, out, logits = half(L, T, 3 * row), half(L, T, row), half(L, T, row), half(T, V)
+    parents = [-1] + [int(rng.integers(max(0, t - 3), t)) for t in range(1, T)]
+    mask, depth = (x.cuda() for x in qdiy.tree_layout(parents))
+    head = dev((0.3 * rng.standard_normal((V, row))).astype(np.float16))
+    tokens, par = torch.zeros(T, dtype=torch.int32, device="cuda"), dev(np.array(parents, np.int32))
+    au, su = torch.empty(T, device="cuda"), torch.empty(1, device="cuda")
+    path, emitted = (torch.empty(T, dtype=torch.int32, device="cuda") for _ in range(2))
+    count = torch.empty(1, dtype=torch.int32, device="cuda")
+    ws = torch.empty(max(ctx.tree_attention_workspace_bytes(T), qdiy.tree_verify_workspace_bytes(T, V)),
+                     dtype=torch.uint8, device="cuda")
+
+    def step():
+        for l in range(L):
+            ctx.tree_qkv_rope(qkv[l], None, depth, q[l], kt[l], vt[l], P, T)
+            ctx.tree_attention(q[l], kc[l], vc[l], kt[l], vt[l], mask, out[l], P, T, ws)
+        qdiy.gemm_nt(out[L - 1], head, logits, T, V, row)
+        qdiy.tree_verify(logits, tokens, par, T, V, ws, path, emitted, count, temperature=0.9, accept_u=au, sample_u=su)
+        ctx.tree_commit(kt, vt, kc, vc, path, count, P, T, layers=L)
+
+    def results():
+        torch.cuda.synchronize()
+        return [x.cpu().numpy().copy() for x in (kc, vc, kt, vt, out, logits, path, emitted, count)]
+
+    def inputs(seed):
+        r = np.random.default_rng(seed)
+        for x in (kc, vc, qkv):
+            x.copy_(dev(r.standard_normal(tuple(x.shape)).astype(np.float16)))
+        start = kc.clone(), vc.clone()
+        au.copy_(dev(0.02 * r.random(T, dtype=np.float32)))
+        su.copy_(dev(r.random(1, dtype=np.float32)))
+        tokens.zero_()
+        step()                                               # drafts: what the target finds likely
+        order = torch.argsort(logits.float(), dim=1, descending=True, stable=True)
+        tokens[1:] = order[par[1:].long(), torch.arange(1, T, device="cuda") % 3].int()
+        for x, x0 in zip((kc, vc), start):                   # without the rows that step committed
+            x.copy_(x0)
+        return start
+
+    inputs(1)
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    counts = []
+    for seed in (10, 20, 30, 40, 50):
+        k0, v0 = inputs(seed)                                # (clones)
+        step()
+        want = results()
+        kc.copy_(k0)
+        vc.copy_(v0)
+        for x in (kt, vt, out, logits):
+            x.fill_(7.0)
+        path.fill_(77)
+        g.replay()
+        for a, b in zip(want, results()):
+            assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
+        n = int(count)
+        walk = verify(logits.cpu().numpy(), tokens.cpu().numpy(), parents, "point", 0.9, au.cpu().numpy(), float(su))
+        assert (path.tolist()[:n], emitted.tolist()[:n]) == walk
+        counts.append(n)
+    assert max(counts) > 1                                   # (the drafts weigh some 0.02 each)

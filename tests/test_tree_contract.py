@@ -245,3 +245,32 @@ def test_max_children_is_not_read_without_drawn_siblings(qdiy, mode, max_childre
     rc = lib.qd_tree_verify(V(at), vocab, draft, vocab, p(0), p(1), p(2), p(3), 0.0 if mode == "greedy" else 0.5, nodes,
                             vocab, max_children, V(at + 16384), wsb, p(4), p(5), p(4), None)
     assert rc == qdiy.QD_EINVAL and b"must not overlap" in lib.qd_last_error()
+
+
+# ------------------------------------------------------------------ tensors that no kernel may be given
+
+def test_tensors_of_another_device_are_refused(qdiy):
+    """A host tensor where device 0 is current, without asking any device."""
+    h = halves(4)
+    with pytest.raises(ValueError, match="x is on cpu, the current device is cuda:0"):
+        qdiy._arg(h, "x", torch.float16, 0, 1)
+    with pytest.raises(ValueError, match="workspace is on cpu, the current device is cuda:0"):
+        qdiy._workspace(h, 0)
+    assert qdiy._arg(h, "x", torch.float16, -1, 4) == h.data_ptr()
+    assert qdiy._workspace(h, -1) == (h.data_ptr(), 8)
+
+
+def test_other_tensors_are_refused(qdiy):
+    h = halves(16).view(4, 4)
+    with pytest.raises(TypeError, match="x must be torch.float32"):
+        qdiy._arg(h, "x", torch.float32, -1, 1)
+    with pytest.raises(ValueError, match="x must be contiguous"):
+        qdiy._arg(h.t(), "x", torch.float16, -1, 1)
+    with pytest.raises(ValueError, match="x holds 16 elements, needs 17"):
+        qdiy._arg(h, "x", torch.float16, -1, 17)
+    for x in ([1.0], None, 3):
+        with pytest.raises(TypeError, match="x must be a torch.Tensor"):
+            qdiy._arg(x, "x", torch.float16, -1, 1)
+    for x in (h.t(), 5):
+        with pytest.raises(TypeError, match="workspace"):
+            qdiy._workspace(x, -1)
