@@ -55,21 +55,28 @@ constexpr double kLeast = -28800.0;                    // 2^-900
 // What a sum may hold of weights that should be 0 (2^24 of 2^-900) counts as 0.
 constexpr double kNothing = 1e-250;
 
-// 2^(j / 32) for j < 32, with j << 15 taken off the high word: adding n << 15 to it gives
-// 2^(n / 32) for n = 32 q + j.
-__device__ const unsigned long long kPow32[32] = {
-    0x3ff0000000000000, 0x3fefd9b0d3158574, 0x3fefb5586cf9890f, 0x3fef9301d0125b51,
-    0x3fef72b83c7d517b, 0x3fef54873168b9aa, 0x3fef387a6e756238, 0x3fef1e9df51fdee1,
-    0x3fef06fe0a31b715, 0x3feef1a7373aa9cb, 0x3feedea64c123422, 0x3feece086061892d,
-    0x3feebfdad5362a27, 0x3feeb42b569d4f82, 0x3feeab07dd485429, 0x3feea47eb03a5585,
-    0x3feea09e667f3bcd, 0x3fee9f75e8ec5f74, 0x3feea11473eb0187, 0x3feea589994cce13,
-    0x3feeace5422aa0db, 0x3feeb737b0cdc5e5, 0x3feec49182a3f090, 0x3feed503b23e255d,
-    0x3feee89f995ad3ad, 0x3feeff76f2fb5e47, 0x3fef199bdd85529c, 0x3fef3720dcef9069,
-    0x3fef5818dcfba487, 0x3fef7c97337b9b5f, 0x3fefa4afa2a490da, 0x3fefd0765b6e4540,
+// 2^(j / 32) for j < 32 as the bits of a double, with j << 15 taken off the high word: adding n << 15
+// to it gives 2^(n / 32) for n = 32 q + j.  Formed by the compiler from the exponential's series (the
+// terms left out are below 2^-70).
+struct Pow32 {
+  unsigned long long bits[32];
 };
+constexpr Pow32 make_pow32() {
+  Pow32 t{};
+  for (int j = 0; j < 32; ++j) {
+    const double x = j * 0.6931471805599453 / 32;      // j ln2 / 32
+    double r = 1.0;
+    for (int k = 20; k > 0; --k) r = 1.0 + r * x / k;
+    t.bits[j] = __builtin_bit_cast(unsigned long long, r) - ((unsigned long long)j << 47);
+  }
+  return t;
+}
+__device__ constexpr Pow32 kPow32 = make_pow32();
 
-// 2^(x / 32), kLeast <= x <= 0, to a relative 2e-12: 2^(n/32) times the series of 2^(f/32)
-// to degree 4 on |f| <= 1/2 (remainder (ln2/64)^5 / 5! = 1.3e-12).
+// 2^(x / 32), kLeast <= x <= 0, to a relative 2e-12, by a table of a few powers as in P. T. P. Tang,
+// "Table-driven implementation of the exponential function in IEEE floating-point arithmetic" (ACM
+// TOMS 15, 1989): 2^(n/32) times the series of 2^(f/32) to degree 4 on |f| <= 1/2 (remainder
+// (ln2/64)^5 / 5! = 1.3e-12).
 // Rounding to n by adding 1.5 * 2^52 leaves it in the low word.  (A series on |f| <= 1/2 of a whole
 // exponent, without the table, takes six fp64 instructions more: the pass over 64 rows of 151936
 // logits 14.2 us against 13.9.)
@@ -204,7 +211,7 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(TreeVerifyParams
     if (!__syncthreads_or(child)) return;
   }
   f16x8u raw = fetch8(row, v0, p.vocab);
-  if (lane < 32) table[lane] = kPow32[lane];           // every wave writes it all, and needs no barrier to read it
+  if (lane < 32) table[lane] = kPow32.bits[lane];      // every wave writes it all, and needs no barrier to read it
 #pragma unroll 1
   for (int r = 0; r < p.runs; ++r) {
     const int v = v0 + kVerifyChunk * r;
@@ -387,7 +394,7 @@ __global__ __launch_bounds__(kThreads) void verify_round_kernel(TreeVerifyParams
   const int tok = child >= 0 ? p.tokens[child] : -1;
   const float u = child >= 0 ? p.accept_u[child] : 0.0f;
   f16x8u xr = fetch8(rp, v0, p.vocab), yr = fetch8(rq, v0, p.vocab);
-  if (threadIdx.x < 32) table[threadIdx.x] = kPow32[threadIdx.x];
+  if (threadIdx.x < 32) table[threadIdx.x] = kPow32.bits[threadIdx.x];
   const bool in = tok >= 0 && tok < p.vocab;
   const float lp = in ? logit(rp, tok) : 0.0f, lq = in ? logit(rq, tok) : 0.0f;
   __syncthreads();
@@ -471,7 +478,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(TreeVerifyPar
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool drawn = !p.greedy && p.draft != nullptr;
   const float sample_u = p.greedy ? 0.0f : *p.sample_u;
-  if (!p.greedy && tid < 32) sh.table[tid] = kPow32[tid];
+  if (!p.greedy && tid < 32) sh.table[tid] = kPow32.bits[tid];
   // Thread t: node t and, on their way while the rows are summed, its token's logits in its
   // parent's rows.
   static_assert(kWalkThreads >= kNodes, "a thread per node");
