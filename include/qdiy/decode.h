@@ -166,11 +166,15 @@ int qd_lm_head_argmax(const uint16_t* x, const uint16_t* norm_w, float eps, cons
  * and the cache changes only when a path is committed.  The context's num_heads
  * is the cache's head count; num_heads here is the number of query heads, a
  * multiple of it: query head h reads cache head h / (num_heads / ctx heads).
- * At most QD_TREE_MAX_NODES nodes.  Counts, depths and paths are device int32,
- * so a step needs no host synchronisation before its next token is wanted.
- * As for the other entry points, calls with distinct workspaces and outputs may
- * run at the same time on several streams; a workspace belongs to one call
- * at a time (two captured graphs that share one must not run together). */
+ * At most QD_TREE_MAX_NODES nodes, 4096 query heads, strides of 2^40 elements.
+ * Depths, paths and counts are device int32, so the calls of one step follow each
+ * other without the host.  prefix is the host's: the next step's is prefix +
+ * count, which the host has to read first, and a captured graph of a step holds
+ * for the prefix that it was captured with, no other.
+ * These calls take only the context's sizes and its cos/sin table: calls with
+ * distinct workspaces and outputs may run at the same time on several streams,
+ * also of one context.  A workspace belongs to one call at a time (two captured
+ * graphs that share one must not run together). */
 #define QD_TREE_MAX_NODES 1024
 
 /* Host only: masks and depths of a tree.  mask[t * ceil(nodes / 64) + w] bit b
@@ -252,11 +256,16 @@ size_t qd_tree_attention_workspace_bytes(const qd_ctx* ctx, int nodes, int num_h
  *   The last token of the two sampled modes is the first index whose cumulative
  *   p exceeds sample_u[0] times its total.
  * In both sampled modes the emitted tokens are distributed as the target's when
- * accept_u and sample_u are independent uniforms of [0, 1).  Weights are held
- * and summed in 64 bits.  A NaN logit counts as -inf; +inf logits share the
+ * accept_u and sample_u are independent uniforms of [0, 1).  Weights are 64-bit
+ * numbers good to a relative 2e-12, and summed in 64 bits; what rejected given
+ * drafts leave for their siblings is 1 less their shares, good to some 1e-11 of
+ * the whole.  (Random numbers nearer to a decision than that may fall to its other
+ * side.)  temperature is 0 or in [1e-6, 1e30], vocab at most 2^24.  A NaN logit counts as -inf; +inf logits share the
  * whole probability; a row of -inf alone is uniform.  A token outside
  * [0, vocab) is never accepted, a node whose parent is not in [0, t) never
- * reached.  If max(p - q, 0) is zero everywhere, p is kept as it was.
+ * reached.  If max(p - q, 0) is zero everywhere, p is kept as it was; if nothing
+ * is left of given drafts' p (numbers of 1 and more can do that), the last token is
+ * 0.
  *   path[nodes]:    the accepted nodes from node 0 on, then -1
  *   emitted[nodes]: the tokens of path[1..], then the last token, then -1
  *   count[0]:       the number of entries of both (1 + accepted drafts)
@@ -284,7 +293,8 @@ size_t qd_tree_verify_workspace_bytes(int nodes, int vocab, int max_children);
  * max_seqlen and entries from `nodes` on are skipped; other rows are left as they
  * were (a cache need not reach past row prefix + nodes).  The node rows may be the cache's own rows from prefix on, in every layer
  * (k_tree == k_cache + prefix*kv_row_stride, v alike, all strides the caches'),
- * with path ascending: the path's rows are then moved up in place.  Otherwise
+ * with path strictly ascending, as qd_tree_verify's is: the path's rows are then
+ * moved up in place.  Otherwise
  * they must not overlap the caches, nor the caches' rows each other (as in
  * qd_tree_qkv_rope; with layers) (QD_EINVAL).  fp16 pointers 16-byte aligned,
  * strides multiples of 8. */

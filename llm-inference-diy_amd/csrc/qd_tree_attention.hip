@@ -2,12 +2,12 @@
 // v_mfma_f32_16x16x32_f16).
 //
 // The query rows of one cache head -- `nodes` times the query heads that share it -- are
-// handled together, so every K/V row is read once for up to 64 of them; with few rows a step
+// handled together, so every K/V row is read once for up to 128 of them; with few rows a step
 // is bound by the cache's bytes.  The keys form tiles of 32 rows: those of the cache, then the
-// node rows, which alone are masked.  A workgroup takes one block of 16 kQ query rows of one
-// cache head and every splits-th group of kW tiles, a tile per wave; its waves keep a softmax
-// state each over all of the block's rows and are folded through LDS at the end.  Several
-// splits leave fp32 partials in the workspace, which a second launch folds.
+// node rows, which alone are masked.  A workgroup takes one block of 16 kQ kQW query rows (16 to
+// 128) of one cache head and every splits-th group of kKW tiles, a tile per key wave; its key
+// waves keep a softmax state each over all of the block's rows and are folded through LDS at the
+// end.  Several splits leave fp32 partials in the workspace, which a second launch folds.
 //
 //   S^T = K Q^T     (M = 16 keys, two tiles; N = 16 queries; K = 128 dims in four steps)
 //   O^T += V^T P^T  (M = 16 dims, eight tiles; N = 16 queries; K = 32 keys)
@@ -29,11 +29,12 @@
 // rows.  A query's reference maximum moves only when a score passes it by more than 2^kLazy:
 // weights stay below 2^kLazy, and the accumulators are scaled in few tiles.
 //
-// Measured on MI355X, 16 cache heads, scan + fold of the splits (kernel time, us):
-//   5 nodes over 512 rows     7.4, one launch: latency (arguments, rows, fold, store)
-//   27 nodes over 8191 rows   14.3 + 3.0; 67 MB of cache at 4.7 TB/s
-//   64 nodes over 32700 rows  53.2 + 4.5; 268 MB at 5.0 TB/s (a large copy reaches 4.9)
-//   250 nodes over 4001 rows  22.4 + 5.9; 387 TFLOP/s: a round of two tiles takes ~2850 cycles,
+// Measured on MI355X, 16 cache heads, scan + fold of the splits (kernel time in a trace, medians of
+// 24 calls, us; a trace adds some 0.5 to the shortest):
+//   5 nodes over 512 rows     8.4, one launch: latency (arguments, rows, fold, store)
+//   27 nodes over 8191 rows   16.1 + 4.1; 67 MB of cache at 4.2 TB/s
+//   64 nodes over 32700 rows  54.6 + 4.9; 268 MB at 4.9 TB/s (a large copy reaches 4.9)
+//   250 nodes over 4001 rows  23.0 + 5.9; 378 TFLOP/s: a round of two tiles takes ~2850 cycles,
 //     of them 1088 on the matrix cores and ~1300 in LDS; half of the rest are the start (two
 //     loads' latency), the fold through LDS (4500 cycles) and the partials (16 MB)
 // Half a round's shift between the two waves of a SIMD, so that one's products run beside the

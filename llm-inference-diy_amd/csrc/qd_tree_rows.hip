@@ -4,7 +4,7 @@
 // Both are bound by a launch's own time at the sizes a step has (a few hundred
 // KB), so each is one launch with 16-byte accesses and nothing shared between
 // threads (MI355X: 5 nodes 2.9 us, 250 nodes of 32 + 16 heads 3.6 us; 4 and 60
-// rows into 24 layers of 16 heads 3.5 and 7.5 us, the latter 24 MB moved at 3.1
+// rows into 24 layers of 16 heads 3.9 and 8.0 us, the latter 24 MB moved at 3.0
 // TB/s).  The rotation is qd_qkv_bias_rope_cache's, operation for operation: fp32
 // products, rounded once each (no contraction), cos and sin from the context's
 // table.

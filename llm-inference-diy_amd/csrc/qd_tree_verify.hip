@@ -21,8 +21,8 @@
 //
 // Measured on MI355X: 64 rows of 151936 logits 13 us (25 instructions per logit are 15 of its 25
 // thousand cycles; the loads' and LDS latency at its two ends the rest) and the one workgroup
-// 11; 27 rows of drawn drafts over 32003 logits 5, four rounds of 5.5-6.7 and 10; the greedy
-// check of 5 rows 3.9 and 4.1.
+// 11; 27 rows of drawn drafts over 32003 logits 5, four rounds of 5.5-6.9 and 10; the greedy
+// check of 5 rows 4.0 and 4.0.
 #include "qd_device.h"
 #include "qd_internal.h"
 #include "qd_tree.h"
