@@ -371,3 +371,122 @@ def test_a_captured_step_holds_for_its_prefix(qdiy):
         assert (path.tolist()[:n], emitted.tolist()[:n]) == walk
         counts.append(n)
     assert max(counts) > 1                                   # (the drafts weigh some 0.02 each)
+
+
+# ------------------------------------------------------------------ one context, several streams; far strides
+
+def test_calls_of_one_context_on_two_streams(qdiy):
+    """The context gives them its sizes and its cos/sin table only."""
+    ctx = qdiy.Context(num_heads=8, max_seqlen=2100)
+    cs = [Attention(qdiy, 8, 8, 2000 + 77 * i, 30, seed=60 + i) for i in range(2)]
+    rope = []
+    for i, c in enumerate(cs):
+        c.ctx = ctx
+        x = dev(np.random.default_rng(70 + i).standard_normal((30, 24 * 128)).astype(np.float16))
+        depth = torch.arange(30, dtype=torch.int32, device="cuda") // 2
+        rope.append((x, depth, [torch.empty(30, 1024, dtype=torch.float16, device="cuda") for _ in range(3)]))
+
+    def call(i, stream=None):
+        cs[i].call(stream=stream)
+        x, depth, outs = rope[i]
+        ctx.tree_qkv_rope(x, None, depth, *outs, 100 + i, 30, stream=stream)
+
+    def got(i):
+        return [t.cpu().numpy().copy() for t in (cs[i].out, *rope[i][2])]
+
+    for i in range(2):
+        call(i)
+    torch.cuda.synchronize()
+    want = [got(i) for i in range(2)]
+    for i in range(2):
+        for t in (cs[i].out[:30], *rope[i][2]):
+            t.zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cs]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            call(i, s)
+    torch.cuda.synchronize()
+    for i in range(2):
+        for a, b in zip(want[i], got(i)):
+            assert np.array_equal(a.view(np.uint16), b.view(np.uint16))
+
+
+def test_heads_and_layers_past_32_bits(qdiy):
+    """Heads and layers 2^31 + 64 elements apart, 4 GiB and a little, in the cache and in the node rows."""
+    far, P, T, S = (1 << 31) + 64, 40, 12, 60
+    c = Attention(qdiy, 2, 2, P, T, seed=80)
+    want = c.result().copy()
+    c.ctx = qdiy.Context(num_heads=2, max_seqlen=S, kv_row_stride=128, kv_head_stride=far)
+    c.trow, c.thead = 128, far
+    big = [torch.empty(2 * far, dtype=torch.float16, device="cuda") for _ in range(4)]
+    c.kc, c.vc, c.kt, c.vt = big
+    rows = lambda x, n: torch.as_strided(x, (n, 2, 128), (128, far, 1))
+    for x, src, n in ((c.kc, c.K, P), (c.vc, c.V, P), (c.kt, c.Kt, T), (c.vt, c.Vt, T)):
+        rows(x, n).copy_(dev(src))
+    assert np.array_equal(want.view(np.uint16), c.result().view(np.uint16))
+    # the path 0, 3, 4 into the cache
+    path, count = dev(np.array([0, 3, 4] + [-1] * (T - 3), np.int32)), dev(np.array([3], np.int32))
+    c.ctx.tree_commit(c.kt, c.vt, c.kc, c.vc, path, count, P, T, tree_row_stride=128, tree_head_stride=far)
+    for x, src, old in ((c.kc, c.Kt, c.K), (c.vc, c.Vt, c.V)):
+        assert np.array_equal(rows(x, P + 3).cpu().numpy(), np.concatenate([old, src[[0, 3, 4]]]))
+    # heads near, layers far
+    ctx = qdiy.Context(num_heads=1, max_seqlen=S)
+    for x in (c.kc, c.vc):
+        torch.as_strided(x, (2, S, 128), (far, 128, 1)).zero_()
+    ctx.tree_commit(c.kt, c.vt, c.kc, c.vc, path, count, P, T, layers=2, tree_layer_stride=far, cache_layer_stride=far)
+    for x, src in ((c.kc, c.Kt), (c.vc, c.Vt)):
+        layers = torch.as_strided(x, (2, S, 128), (far, 128, 1))
+        for l in range(2):
+            assert torch.equal(layers[l, P:P + 3], dev(src[[0, 3, 4], l]))
+            assert not layers[l, :P].any() and not layers[l, P + 3:].any()
+    # node rows from RoPE, heads far
+    x = dev(np.random.default_rng(81).standard_normal((T, 6 * 128)).astype(np.float16))
+    depth = torch.arange(T, dtype=torch.int32, device="cuda") // 3
+    near = [torch.empty(T, 256, dtype=torch.float16, device="cuda") for _ in range(3)]
+    q = torch.empty(T, 256, dtype=torch.float16, device="cuda")
+    c.ctx.tree_qkv_rope(x, None, depth, *near, 7, T)
+    c.ctx.tree_qkv_rope(x, None, depth, q, c.kt, c.vt, 7, T, tree_row_stride=128, tree_head_stride=far)
+    assert torch.equal(q, near[0])
+    for a, b in ((c.kt, near[1]), (c.vt, near[2])):
+        assert torch.equal(rows(a, T), b.view(T, 2, 128))
+
+
+# ------------------------------------------------------------------ the largest calls
+
+@pytest.mark.parametrize("H,T,P", [(4095, 1024, 33), (4096, 1023, 700)])
+def test_the_most_query_rows(qdiy, H, T, P):
+    """Four million query rows of one cache head; a float64 sample of nodes and heads, within the
+    bound of the kernel's roundings."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(H)
+    half = lambda *n: torch.randn(*n, generator=g, device="cuda").half()
+    q = torch.empty(T, H * 128, dtype=torch.float16, device="cuda")
+    for t0 in range(0, T, 128):
+        q[t0:t0 + 128] = half(min(128, T - t0), H * 128)
+    k, v, kt, vt = half(P, 128), half(P, 128), half(T, 128), half(T, 128)
+    parents = [-1] + [max(0, t - 1 - t % 7) for t in range(1, T)]
+    mask = qdiy.tree_layout(parents)[0].cuda()
+    ctx = qdiy.Context(num_heads=1, max_seqlen=P)
+    ws = torch.empty(ctx.tree_attention_workspace_bytes(T, H), dtype=torch.uint8, device="cuda")
+    out = torch.full((T, H * 128), 7.0, dtype=torch.float16, device="cuda")
+    ctx.tree_attention(q, k, v, kt, vt, mask, out, P, T, ws, num_heads=H)
+    assert bool(torch.isfinite(out).all())
+    vis = ancestors(parents)
+    nodes = sorted({0, 1, T // 3, T // 2, T - 2, T - 1})
+    host = lambda x: x.cpu().numpy()
+    for h in sorted({0, 1, 63, 64, H // 2, H - 2, H - 1}):
+        cols = slice(h * 128, h * 128 + 128)
+        # (a node's row of vis names all node rows that it sees)
+        for t in nodes:
+            want, bound = attention(host(q[t:t + 1, cols])[:, None], host(k)[:, None], host(v)[:, None], host(kt)[:, None],
+                                    host(vt)[:, None], vis[t:t + 1], with_bound=True)
+            err = np.abs(host(out[t, cols]).astype(np.float64) - want[0, 0])
+            assert np.all(err <= bound[0, 0]), (h, t)
+
+
+@pytest.mark.parametrize("mode", ["greedy", "point", "drawn"])
+@pytest.mark.parametrize("T,V", [(300, 40001), (1024, 9000)])
+def test_many_rows_whose_chunks_share_workgroups(qdiy, mode, T, V):
+    for seed in range(2):
+        Verify(T, V, mode, seed=seed).check(qdiy)
